@@ -17,8 +17,10 @@ from .chunk_layout import (  # noqa: F401
     register_param,
 )
 from .client import PatrickStarClient, plan_host_positions  # noqa: F401
+from .distill import TopLogits, distill_loss, top_logits  # noqa: F401
 from .engine import PatrickStarEngine, initialize_engine, parse_config  # noqa: F401
 from .fp16_adam import FP16Adam  # noqa: F401
 from .loss_scaler import DynamicLossScaler, LossScaler  # noqa: F401
+from .rotary import RotaryPlan, norm_rotate_qk, rotate_qk  # noqa: F401
 
 __version__ = "0.1.0"

@@ -17,6 +17,8 @@ PS_ARITH_OPERATOR, PS_ARITH_TORCH = 0, 1
 PS_TENSOR_GRAD_F32 = 1
 PS_ABI_VERSION = 5
 PS_STEP_SCRATCH_BYTES = 448
+PS_F16, PS_BF16, PS_F32 = 0, 1, 2
+PS_MAX_HEAD_DIM, PS_MAX_TOP = 512, 1024
 
 
 class ps_chunk(ctypes.Structure):
@@ -103,6 +105,85 @@ class ps_grad_copy(ctypes.Structure):
     ]
 
 
+class ps_heads_call(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p * 2),
+        ("grad", ctypes.c_void_p * 2),
+        ("out", ctypes.c_void_p * 2),
+        ("weight", ctypes.c_void_p * 2),
+        ("weight_grad", ctypes.c_void_p * 2),
+        ("positions", ctypes.c_void_p),
+        ("plan", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64 * 6),
+        ("grad_stride", ctypes.c_int64 * 6),
+        ("position_stride", ctypes.c_int64 * 3),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int32 * 2),
+        ("dim", ctypes.c_int32),
+        ("rotary", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("position_bytes", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32 * 2),
+    ]
+
+
+class ps_top_call(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("ids", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("k", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class ps_distill_call(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("ids", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("teacher_lse", ctypes.c_void_p),
+        ("labels", ctypes.c_void_p),
+        ("row_loss", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("loss", ctypes.c_void_p),
+        ("denominator", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("upstream", ctypes.c_void_p),
+        ("upstream_used", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("ids_stride", ctypes.c_int64),
+        ("values_stride", ctypes.c_int64),
+        ("upstream_stride", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("k", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("values_dtype", ctypes.c_int32),
+        ("ids_bytes", ctypes.c_int32),
+        ("labels_bytes", ctypes.c_int32),
+        ("mean", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("label_weight", ctypes.c_float),
+        ("upstream_value", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class ps_scale_record(ctypes.Structure):
     _fields_ = [
         ("scale_after", ctypes.c_double),
@@ -117,6 +198,9 @@ assert ctypes.sizeof(ps_call_pattern) == 32
 assert ctypes.sizeof(ps_scale_record) == 16
 assert ctypes.sizeof(ps_tensor_call) == 56
 assert ctypes.sizeof(ps_grad_copy) == 32
+assert ctypes.sizeof(ps_heads_call) == 288
+assert ctypes.sizeof(ps_top_call) == 72
+assert ctypes.sizeof(ps_distill_call) == 192
 
 _f, _d, _i, _i64, _sz, _vp = (
     ctypes.c_float,
@@ -162,6 +246,16 @@ SIGNATURES = {
     "ps_state_read": (_i, [_vp, ctypes.POINTER(ps_step_state), _vp]),
 }
 
+# the same of include/ps_ops.h; descriptors are passed by address
+OP_SIGNATURES = {
+    "ps_rotate_heads": (_i, [_vp, _vp]),
+    "ps_norm_rotate_heads_workspace_bytes": (_sz, [_vp]),
+    "ps_norm_rotate_heads_backward": (_i, [_vp, _vp, _sz, _vp]),
+    "ps_top_logits": (_i, [_vp, _vp]),
+    "ps_distill_loss": (_i, [_vp, _vp]),
+    "ps_distill_loss_backward": (_i, [_vp, _vp]),
+}
+
 _lib = None
 
 
@@ -184,7 +278,7 @@ def load():
     version = lib.ps_abi_version() if hasattr(lib, "ps_abi_version") else "none"
     if version != PS_ABI_VERSION:
         raise HipLibraryMissing(f"{LIB_PATH} has ABI version {version}, expected {PS_ABI_VERSION}; rebuild it")
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in (*SIGNATURES.items(), *OP_SIGNATURES.items()):
         fn = getattr(lib, name, None)
         if fn is None:
             raise HipLibraryMissing(f"{LIB_PATH} has no {name}: it is older than this package; rebuild it")
@@ -248,6 +342,11 @@ def check(rc, what):
     if rc != 0:
         msg = load().ps_last_error()
         raise RuntimeError(f"{what} failed (code {rc}): {msg.decode() if msg else ''}")
+
+
+def address(structure):
+    """Where a descriptor lies, as the entry points take it."""
+    return ctypes.addressof(structure)
 
 
 def raw_stream(device):

@@ -8,7 +8,7 @@ import sys
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 LIB_PATH = os.path.join(PKG_DIR, "libps_adam.so")
-SOURCES = [os.path.join(PKG_DIR, "csrc", "ps_adam.hip")]
+SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("ps_adam.hip", "ps_ops.hip")]
 BINDING_SOURCE = os.path.join(PKG_DIR, "csrc", "ps_binding.cpp")
 BINDING_PATH = os.path.join(PKG_DIR, "_binding.so")
 INCLUDE = os.path.join(ROOT, "include")

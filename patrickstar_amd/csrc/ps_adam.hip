@@ -54,35 +54,12 @@
 #include "ps_adam.h"
 
 #include "ps_config.h"
+#include "ps_error.h"
 #include "ps_arith.h"
 #include "ps_tile.h"
 #include "ps_kernels.h"
 
 namespace {
-
-// ------------------------------------------------------------------ errors
-
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...)
-{
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    return code;
-}
-
-int hip_fail(hipError_t e, const char* what)
-{
-    return fail(-(int)e, "%s: %s", what, hipGetErrorString(e));
-}
-
-#define PS_HIP(call)                                      \
-    do {                                                  \
-        hipError_t e_ = (call);                           \
-        if (e_ != hipSuccess) return hip_fail(e_, #call); \
-    } while (0)
 
 // ------------------------------------------------------- host scalar state
 //
@@ -900,7 +877,7 @@ extern "C" {
 
 int ps_abi_version(void) { return PS_ABI_VERSION; }
 
-const char* ps_last_error(void) { return g_err; }
+const char* ps_last_error(void) { return ps_detail::error_text; }
 
 int ps_adam_create(int optimizer_id, float alpha, float beta1, float beta2, float eps,
                    float weight_decay, int adamw_mode, int should_log)

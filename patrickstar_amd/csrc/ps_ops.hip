@@ -1,0 +1,370 @@
+// The C ABI of include/ps_ops.h: checks of the descriptors, launch shapes, launches.  Kernels: ps_rotary.h, ps_logits.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "ps_ops.h"
+
+#include "ps_error.h"
+#include "ps_rotary.h"
+#include "ps_logits.h"
+
+namespace {
+
+constexpr int kCus = 256;
+
+int size_of(int dtype) { return dtype == PS_F32 ? 4 : 2; }
+
+bool known(int dtype) { return dtype == PS_F16 || dtype == PS_BF16 || dtype == PS_F32; }
+
+// Calls f(a value of the element type).
+template <typename F>
+void with_type(int dtype, F f)
+{
+    if (dtype == PS_F16)
+        f(half_t());
+    else if (dtype == PS_BF16)
+        f(bf16_t());
+    else
+        f(float());
+}
+
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// ---------------------------------------------------------------------------------------------------------- rotations
+
+int check_heads(const ps_heads_call* c, bool backward)
+{
+    if (!c) return fail(PS_ERR_BAD_ARG, "call is NULL");
+    if (!known(c->dtype)) return fail(PS_ERR_BAD_ARG, "dtype %d is unknown", c->dtype);
+    if (c->weight_dtype != c->dtype && c->weight_dtype != PS_F32)
+        return fail(PS_ERR_BAD_ARG, "weight_dtype %d: the elements' own type or PS_F32", c->weight_dtype);
+    if (c->position_bytes != 4 && c->position_bytes != 8) return fail(PS_ERR_BAD_ARG, "position_bytes = %d", c->position_bytes);
+    if (c->dim < 1 || c->dim > PS_MAX_HEAD_DIM) return fail(PS_ERR_BAD_ARG, "dim = %d is not in 1 .. %d", c->dim, PS_MAX_HEAD_DIM);
+    if (c->rotary < 0 || c->rotary % 2 || c->rotary > c->dim)
+        return fail(PS_ERR_BAD_ARG, "rotary = %d must be even and at most dim = %d", c->rotary, c->dim);
+    if (c->axes < 1) return fail(PS_ERR_BAD_ARG, "axes = %d", c->axes);
+    if (c->batch < 0 || c->tokens < 0 || c->heads[0] < 0 || c->heads[1] < 0) return fail(PS_ERR_BAD_ARG, "a negative size");
+    if (c->heads[0] > (1 << 20) || c->heads[1] > (1 << 20)) return fail(PS_ERR_BAD_ARG, "more than 2^20 heads");
+    if (c->tokens && c->batch > INT32_MAX / c->tokens) return fail(PS_ERR_BAD_ARG, "more than 2^31 - 1 tokens");
+    if (!(c->eps >= 0.0f)) return fail(PS_ERR_BAD_ARG, "eps = %g", (double)c->eps);
+    if (c->batch * c->tokens == 0) return 0;
+    for (int w = 0; w < 2; ++w) {
+        if (c->heads[w] == 0) continue;
+        if (!c->x[w] || !c->out[w] || (backward && !c->grad[w])) return fail(PS_ERR_BAD_ARG, "%s have a NULL address", w ? "keys" : "queries");
+        const uintptr_t bytes = (uintptr_t)size_of(c->dtype);
+        if ((uintptr_t)c->x[w] % bytes || (uintptr_t)c->out[w] % bytes || (backward && (uintptr_t)c->grad[w] % bytes))
+            return fail(PS_ERR_BAD_ARG, "%s are not aligned to their type", w ? "keys" : "queries");
+        if (c->weight_grad[w] && !c->weight[w]) return fail(PS_ERR_BAD_ARG, "a gradient is wanted of a weight that is not there");
+    }
+    if (c->rotary && (!c->positions || !c->plan)) return fail(PS_ERR_BAD_ARG, "positions or plan is NULL");
+    return 0;
+}
+
+// Whether every vector of `v` elements that a kernel touches lies at a multiple of its size.
+bool fits_vectors(const ps_heads_call* c, int v, bool backward)
+{
+    if (c->dim % v || (c->rotary / 2) % v) return false;
+    const uintptr_t bytes = (uintptr_t)v * size_of(c->dtype);
+    for (int w = 0; w < 2; ++w) {
+        if (c->heads[w] == 0) continue;
+        if ((uintptr_t)c->x[w] % bytes || (uintptr_t)c->out[w] % bytes) return false;
+        for (int i = 0; i < 3; ++i)
+            if (c->x_stride[w][i] % v) return false;
+        if (!backward) continue;
+        if ((uintptr_t)c->grad[w] % bytes) return false;
+        for (int i = 0; i < 3; ++i)
+            if (c->grad_stride[w][i] % v) return false;
+    }
+    return true;
+}
+
+struct HeadsShape {
+    HeadsArgs a;
+    int v;               // elements of a vector
+    uint32_t waves;      // that the call's tokens take
+    uint32_t splits;     // of a token's heads
+};
+
+HeadsShape heads_shape(const ps_heads_call* c, bool backward)
+{
+    HeadsShape s;
+    HeadsArgs& a = s.a;
+    memset(&a, 0, sizeof(a));
+    memcpy(a.x, c->x, sizeof(a.x));
+    memcpy(a.grad, c->grad, sizeof(a.grad));
+    memcpy(a.out, c->out, sizeof(a.out));
+    memcpy(a.weight, c->weight, sizeof(a.weight));
+    memcpy(a.x_stride, c->x_stride, sizeof(a.x_stride));
+    memcpy(a.grad_stride, c->grad_stride, sizeof(a.grad_stride));
+    memcpy(a.position_stride, c->position_stride, sizeof(a.position_stride));
+    memcpy(a.heads, c->heads, sizeof(a.heads));
+    a.positions = c->positions;
+    a.plan = c->plan;
+    a.tokens = (uint32_t)c->tokens;
+    a.all_tokens = (uint32_t)(c->batch * c->tokens);
+    a.dim = c->dim;
+    a.pairs = c->rotary / 2;
+    a.eps = c->eps;
+    a.inv_dim = 1.0f / (float)c->dim;
+    a.weight_f32 = c->weight_dtype == PS_F32;
+    a.positions_64 = c->position_bytes == 8;
+    a.interleaved = c->interleaved != 0;
+    a.inverse = c->inverse != 0;
+    s.v = 16 / size_of(c->dtype);
+    while (!fits_vectors(c, s.v, backward)) s.v /= 2;
+    const int units = (c->dim + 2 * s.v - 1) / (2 * s.v);
+    while ((1 << a.group_shift) < units && a.group_shift < 6) ++a.group_shift;
+    const int heads = c->heads[0] + c->heads[1];
+    while ((1 << a.slot_shift) < heads && a.slot_shift < 6 - a.group_shift) ++a.slot_shift;
+    const int tokens_shift = 6 - a.group_shift - a.slot_shift;
+    s.waves = (a.all_tokens + (1u << tokens_shift) - 1) >> tokens_shift;
+    // few tokens: a token's heads are spread over more waves, each of which makes the token's angles for itself
+    const uint32_t turns = (uint32_t)((heads + (1 << a.slot_shift) - 1) >> a.slot_shift);
+    s.splits = 1;
+    while (s.splits < turns && s.waves * s.splits < 4 * kCus) s.splits *= 2;
+    s.splits = std::min({s.splits, turns, 65535u});
+    return s;
+}
+
+// Calls f(type, vector length, units a lane).
+template <typename F>
+void with_heads_kernel(int dtype, int v, F f)
+{
+    with_type(dtype, [&](auto t) {
+        if constexpr (sizeof(t) == 2) {
+            if (v == 8) return f(t, Int<8>(), Int<1>());
+        }
+        if (v == 4) return f(t, Int<4>(), Int<1>());
+        if (v == 2) return f(t, Int<2>(), Int<2>());
+        f(t, Int<1>(), Int<4>());
+    });
+}
+static_assert(PS_MAX_HEAD_DIM <= 2 * 4 * 64 && PS_MAX_HEAD_DIM <= 2 * 2 * 2 * 64 && PS_MAX_HEAD_DIM <= 2 * 64 * 4, "a group holds a head");
+
+uint32_t backward_blocks(const HeadsShape& s)
+{
+    const uint32_t blocks = (s.waves + kHeadsBlock / 64 - 1) / (kHeadsBlock / 64);
+    return std::min(blocks, std::max(1u, 4u * kCus / s.splits));
+}
+
+bool wants_weight_grad(const ps_heads_call* c)
+{
+    return (c->weight_grad[0] && c->heads[0]) || (c->weight_grad[1] && c->heads[1]);
+}
+
+// ------------------------------------------------------------------------------------------------------------- logits
+
+// Calls f(vectors a thread keeps, threads): the shortest row that holds the vocabulary; 0 where none does.
+template <typename T, typename F>
+void with_row(int vocab, bool wide, F f)
+{
+    const int vectors = vocab / (16 / (int)sizeof(T)) + 1;
+    if (!wide) {
+        if (vectors <= 256) return f(Int<1>(), Int<256>());
+        if (vectors <= 512) return f(Int<2>(), Int<256>());
+        if (vectors <= 1024) return f(Int<4>(), Int<256>());
+        if (vectors <= 2048) return f(Int<8>(), Int<256>());
+    }
+    if (vectors <= 2048) return f(Int<2>(), Int<1024>());
+    if (vectors <= 4096) return f(Int<4>(), Int<1024>());
+    if (vectors <= 8192) return f(Int<8>(), Int<1024>());
+    if (vectors <= 16384) return f(Int<16>(), Int<1024>());
+    f(Int<0>(), Int<1024>());
+}
+
+unsigned row_blocks(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 21); }
+
+constexpr int64_t kMaxTopVocab = 1 << 30;
+constexpr int64_t kMaxDistillVocab = 400000;  // a bit each in LDS, beside a list
+
+int check_rows(int64_t rows, int64_t vocab, int64_t most, int dtype, const void* logits, int k)
+{
+    if (!known(dtype)) return fail(PS_ERR_BAD_ARG, "dtype %d is unknown", dtype);
+    if (rows < 0) return fail(PS_ERR_BAD_ARG, "rows = %lld is negative", (long long)rows);
+    if (vocab < 1 || vocab > most) return fail(PS_ERR_BAD_ARG, "vocab = %lld is not in 1 .. %lld", (long long)vocab, (long long)most);
+    if (k < 1 || k > PS_MAX_TOP) return fail(PS_ERR_BAD_ARG, "k = %d is not in 1 .. %d", k, PS_MAX_TOP);
+    if (rows && !logits) return fail(PS_ERR_BAD_ARG, "logits is NULL");
+    if ((uintptr_t)logits % size_of(dtype)) return fail(PS_ERR_BAD_ARG, "logits is not aligned to its type");
+    return 0;
+}
+
+bool positive(float t) { return t > 0.0f && std::isfinite(t); }
+
+int distill_args(const ps_distill_call* c, bool backward, DistillArgs& a)
+{
+    if (!c) return fail(PS_ERR_BAD_ARG, "call is NULL");
+    if (int rc = check_rows(c->rows, c->vocab, kMaxDistillVocab, c->dtype, c->logits, c->k)) return rc;
+    if (!known(c->values_dtype)) return fail(PS_ERR_BAD_ARG, "values_dtype %d is unknown", c->values_dtype);
+    if (c->ids_bytes != 4 && c->ids_bytes != 8) return fail(PS_ERR_BAD_ARG, "ids_bytes = %d", c->ids_bytes);
+    if (c->labels && c->labels_bytes != 4 && c->labels_bytes != 8) return fail(PS_ERR_BAD_ARG, "labels_bytes = %d", c->labels_bytes);
+    if (!positive(c->temperature)) return fail(PS_ERR_BAD_ARG, "temperature = %g must be positive", (double)c->temperature);
+    if (!(c->label_weight >= 0.0f && c->label_weight <= 1.0f))
+        return fail(PS_ERR_BAD_ARG, "label_weight = %g is not in 0 .. 1", (double)c->label_weight);
+    if (c->label_weight > 0.0f && !c->labels) return fail(PS_ERR_BAD_ARG, "label_weight without labels");
+    if (c->rows && (!c->ids || !c->values)) return fail(PS_ERR_BAD_ARG, "the teacher's list is NULL");
+    if (c->rows && !backward && !c->row_loss) return fail(PS_ERR_BAD_ARG, "row_loss is NULL");
+    if (c->rows && backward && (!c->grad || !c->stats || !c->upstream)) return fail(PS_ERR_BAD_ARG, "grad, stats or upstream is NULL");
+    if (c->mean && !c->denominator) return fail(PS_ERR_BAD_ARG, "a mean needs the denominator's place");
+    memset(&a, 0, sizeof(a));
+    a.logits = c->logits;
+    a.ids = c->ids;
+    a.values = c->values;
+    a.teacher_lse = c->teacher_lse;
+    a.labels = c->labels;
+    a.row_loss = c->row_loss;
+    a.stats = c->stats;
+    a.denominator = c->mean ? c->denominator : nullptr;
+    a.grad = c->grad;
+    a.upstream = c->upstream;
+    a.upstream_used = c->upstream_used;
+    a.rows = c->rows;
+    a.row_stride = c->row_stride;
+    a.ids_stride = c->ids_stride;
+    a.values_stride = c->values_stride;
+    a.upstream_stride = c->upstream_stride;
+    a.ignore_index = c->ignore_index;
+    a.vocab = (int)c->vocab;
+    a.k = c->k;
+    a.values_dtype = c->values_dtype;
+    a.temperature = c->temperature;
+    a.label_weight = c->label_weight;
+    a.upstream_value = c->upstream_value;
+    a.ids_64 = c->ids_bytes == 8;
+    a.labels_64 = c->labels_bytes == 8;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ps_rotate_heads(const ps_heads_call* call, ps_stream_t stream)
+{
+    if (int rc = check_heads(call, false)) return rc;
+    if (call->batch * call->tokens == 0 || call->heads[0] + call->heads[1] == 0) return 0;
+    const HeadsShape s = heads_shape(call, false);
+    const dim3 grid((s.waves + kHeadsBlock / 64 - 1) / (kHeadsBlock / 64), s.splits);
+    with_heads_kernel(call->dtype, s.v, [&](auto t, auto v, auto u) {
+        typedef decltype(t) T;
+        if (call->norm)
+            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), true>), grid, dim3(kHeadsBlock), 0, static_cast<hipStream_t>(stream), s.a);
+        else
+            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), false>), grid, dim3(kHeadsBlock), 0, static_cast<hipStream_t>(stream), s.a);
+    });
+    PS_HIP(hipGetLastError());
+    return 0;
+}
+
+size_t ps_norm_rotate_heads_workspace_bytes(const ps_heads_call* call)
+{
+    if (check_heads(call, true) || call->batch * call->tokens == 0 || !wants_weight_grad(call)) return 0;
+    const HeadsShape s = heads_shape(call, true);
+    return (size_t)backward_blocks(s) * s.splits * 2 * (size_t)call->dim * sizeof(float);
+}
+
+int ps_norm_rotate_heads_backward(const ps_heads_call* call, void* d_workspace, size_t workspace_bytes, ps_stream_t stream)
+{
+    if (int rc = check_heads(call, true)) return rc;
+    const size_t needed = ps_norm_rotate_heads_workspace_bytes(call);
+    if (workspace_bytes < needed || (needed && (!d_workspace || (uintptr_t)d_workspace % 16)))
+        return fail(PS_ERR_BAD_ARG, "the workspace has %zu bytes at %p, %zu are needed, 16-byte aligned", workspace_bytes, d_workspace, needed);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool empty = call->batch * call->tokens == 0;
+    uint32_t rows = 0;
+    if (!empty && call->heads[0] + call->heads[1] > 0) {
+        HeadsShape s = heads_shape(call, true);
+        s.a.inverse = !call->inverse;  // the gradient turns back
+        s.a.partial = needed ? static_cast<float*>(d_workspace) : nullptr;
+        const dim3 grid(backward_blocks(s), s.splits);
+        rows = needed ? grid.x * grid.y : 0;
+        with_heads_kernel(call->dtype, s.v, [&](auto t, auto v, auto u) {
+            typedef decltype(t) T;
+            hipLaunchKernelGGL((norm_rotate_heads_backward_kernel<T, v(), u()>), grid, dim3(kHeadsBlock), 0, st, s.a, s.waves);
+        });
+        PS_HIP(hipGetLastError());
+    }
+    if (call->weight_grad[0] || call->weight_grad[1]) {  // (of no tokens: zeros)
+        with_type(call->dtype, [&](auto t) {
+            typedef decltype(t) T;
+            hipLaunchKernelGGL((sum_weight_grads_kernel<T>), dim3((2 * call->dim + kSumColumns - 1) / kSumColumns), dim3(kSumColumns * kSumSlices),
+                               0, st, static_cast<const float*>(d_workspace), (int)rows, call->dim, call->weight_grad[0], call->weight_grad[1],
+                               call->weight_dtype == PS_F32);
+        });
+        PS_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+int ps_top_logits(const ps_top_call* call, ps_stream_t stream)
+{
+    if (!call) return fail(PS_ERR_BAD_ARG, "call is NULL");
+    if (int rc = check_rows(call->rows, call->vocab, kMaxTopVocab, call->dtype, call->logits, call->k)) return rc;
+    if (call->k > call->vocab) return fail(PS_ERR_BAD_ARG, "k = %d is more than the vocabulary of %lld", call->k, (long long)call->vocab);
+    if (!positive(call->temperature)) return fail(PS_ERR_BAD_ARG, "temperature = %g must be positive", (double)call->temperature);
+    if (call->rows == 0) return 0;
+    if (!call->values || !call->ids || !call->lse) return fail(PS_ERR_BAD_ARG, "values, ids or lse is NULL");
+    TopArgs a;
+    a.logits = call->logits;
+    a.values = call->values;
+    a.ids = call->ids;
+    a.lse = call->lse;
+    a.rows = call->rows;
+    a.row_stride = call->row_stride;
+    a.vocab = (int)call->vocab;
+    a.k = call->k;
+    a.factor = (float)(1.4426950408889634 / (double)call->temperature);
+    a.temperature = call->temperature;
+    with_type(call->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        with_row<T>(a.vocab, a.k > 128, [&](auto nv, auto block) {
+            hipLaunchKernelGGL((top_logits_kernel<T, nv(), block()>), dim3(row_blocks(a.rows)), dim3(block()), 0, static_cast<hipStream_t>(stream), a);
+        });
+    });
+    PS_HIP(hipGetLastError());
+    return 0;
+}
+
+int ps_distill_loss(const ps_distill_call* call, ps_stream_t stream)
+{
+    DistillArgs a;
+    if (int rc = distill_args(call, false, a)) return rc;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (call->mean) {
+        hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, st, call->labels, a.labels_64, a.rows, a.ignore_index, call->denominator);
+        PS_HIP(hipGetLastError());
+    }
+    if (a.rows) {
+        const unsigned lds = 4u * (unsigned)((a.vocab + 31) / 32) + 8u * (unsigned)a.k;
+        with_type(call->dtype, [&](auto t) {
+            typedef decltype(t) T;
+            with_row<T>(a.vocab, false, [&](auto nv, auto block) {
+                hipLaunchKernelGGL((distill_loss_kernel<T, nv(), block()>), dim3(row_blocks(a.rows)), dim3(block()), lds, st, a);
+            });
+        });
+        PS_HIP(hipGetLastError());
+    }
+    if (call->loss) {
+        hipLaunchKernelGGL(sum_rows_kernel, dim3(1), dim3(1024), 0, st, call->row_loss, a.rows, a.denominator, call->loss);
+        PS_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+int ps_distill_loss_backward(const ps_distill_call* call, ps_stream_t stream)
+{
+    DistillArgs a;
+    if (int rc = distill_args(call, true, a)) return rc;
+    if (a.rows == 0) return 0;
+    with_type(call->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((distill_backward_kernel<T, 256>), dim3(row_blocks(a.rows)), dim3(256), 8u * (unsigned)a.k, static_cast<hipStream_t>(stream), a);
+    });
+    PS_HIP(hipGetLastError());
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,401 @@
+"""Top logits and the distillation loss against their formulas in 64 bits.
+
+Tolerances.  What is chosen has to be equal.  A log-sum-exp: an exponent's error is the rounding of its argument, |z| / T * 2**-23 or so for the
+terms that count (|z| / T up to 40 here: 2**-18), the sum's own error less, and the result is rounded to 24 bits.  A loss is a sum of such
+numbers weighted by probabilities; a gradient's terms are probabilities with a relative error of the same 2**-17 (two exponents, a
+quotient), the share off the list with that of 1 - rest / q_rest, whose rest = 1 - sum(p) has an absolute error of 2**-20 or so from the
+list's k roundings.  Then one rounding to the type."""
+import math
+
+import pytest
+import torch
+
+import patrickstar_amd as ps
+
+pytestmark = pytest.mark.gpu
+
+HALF_ULP = {torch.half: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float: 2.0**-24}
+TINY = {torch.half: 2.0**-25, torch.bfloat16: 0.0, torch.float: 0.0}
+DTYPES = list(HALF_ULP)
+SLACK = 2.0**-17
+
+
+def made(shape, dtype, seed, std=3.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.empty(shape, device="cuda").normal_(0, std, generator=gen).to(dtype)
+
+
+def top_reference(z, k):
+    """By sorting whole numbers in the order of the values, lower places first."""
+    rows = []
+    for row in z.float().cpu():
+        order = sorted(range(len(row)), key=lambda i: (0 if math.isnan(row[i]) else 1, -float(row[i]) if not math.isnan(row[i]) else 0.0, i))
+        rows.append(order[:k])
+    return torch.tensor(rows, dtype=torch.int32, device=z.device)
+
+
+def check_top(z, k, temperature=1.0):
+    values, ids, lse = ps.top_logits(z, k, temperature)
+    want = top_reference(z.reshape(-1, z.shape[-1]), k).view(*z.shape[:-1], k)
+    assert ids.dtype == torch.int32 and torch.equal(ids, want)
+    taken = z.gather(-1, want.long())
+    assert values.dtype == z.dtype and torch.equal(values.nan_to_num(1e4), taken.nan_to_num(1e4)) and torch.equal(values.isnan(), taken.isnan())
+    x = z.double() / temperature
+    exact = x.logsumexp(-1)
+    same = (lse.double() - exact).abs() <= 2.0**-17 * (1 + exact.abs())
+    assert (same | (lse == exact) | (lse.isnan() & exact.isnan())).all(), (lse, exact)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,k", [
+    (1, 1, 1), (3, 2, 2), (2, 7, 3), (5, 64, 64), (4, 257, 16), (3, 1001, 128), (3, 2049, 129), (2, 4099, 1), (2, 16391, 200), (1, 8192, 1024),
+    (2, 30522, 32), (2, 50257, 64), (1, 140003, 100),
+])
+def test_top_logits(rows, vocab, k, dtype):
+    check_top(made((rows, vocab), dtype, rows + vocab), k, 1.0 if vocab % 2 else 2.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_top_logits_of_equal_and_special_numbers(dtype):
+    v = 20011
+    z = made((10, v), dtype, 5)
+    z[0] = 0.5  # all equal
+    z[1] = -math.inf  # nothing allowed
+    z[2, 5:] = -math.inf  # five allowed
+    z[3] = -math.inf
+    z[3, 777] = 1.0
+    z[4, 100], z[4, 19000] = math.inf, math.inf
+    z[5, 50], z[5, 15000] = math.nan, -math.nan
+    z[6] = 0.0
+    z[6, ::3] = -0.0
+    z[7] = torch.where(torch.arange(v, device="cuda") % 2 == 0, 3.0, -3.0)
+    z[8] = -65504.0 if dtype == torch.half else -3e38  # the type's lowest
+    z[8, 9000] = 0.0
+    z[9] = made((v,), dtype, 6, 2.0**-20 if dtype != torch.half else 2.0**-22)  # close to nothing
+    for k in (1, 6, 64, 500):
+        check_top(z, k)
+
+
+def test_top_logits_with_a_stride_and_dimensions():
+    whole = made((3, 4, 1040), torch.half, 8)
+    z = whole[..., 5:1008]
+    check_top(z, 12)
+    check_top(whole.transpose(0, 2)[:16], 2)  # a row's elements apart
+    check_top(whole[0, 0], 5)  # one row, no dimension in front
+    values, ids, lse = ps.top_logits(z[:0], 12)
+    assert values.shape == (0, 4, 12) and ids.shape == (0, 4, 12) and lse.shape == (0, 4)
+    check_top(z[:1, :1].expand(2, 3, 1003), 7)
+
+
+# -------------------------------------------------------------------------------------------------------- distillation
+
+
+def reference(z, ids, t, lse, labels, a, temperature, ignore=-100):
+    """Row losses and their gradients in 64 bits, and the size that the gradients' errors go by."""
+    n, v = z.shape
+    z, t = z.double(), t.double() / temperature
+    q, log_q = (z / temperature).softmax(-1), (z / temperature).log_softmax(-1)
+    there = ids >= 0
+    slot = torch.where(there, ids.long(), v)
+    p = torch.zeros(n, v + 1, dtype=torch.float64, device=z.device)
+    on = torch.zeros_like(p)
+    on.scatter_(1, slot, 1.0)
+    if lse is None:
+        p.scatter_(1, slot, t.masked_fill(~there, -math.inf).softmax(-1).nan_to_num(0.0))
+    else:
+        p.scatter_(1, slot, (t - lse.double()[:, None]).exp())
+    p, on = p[:, :v], on[:, :v]
+    mass = p.sum(1, keepdim=True)
+    loss = torch.where(p > 0, torch.xlogy(p, p) - p * log_q, 0.0).sum(1)
+    grad = q * mass - p
+    size = q * mass + p
+    if lse is not None:
+        rest = (1 - mass).clamp(min=0)
+        q_rest = (q * (1 - on)).sum(1, keepdim=True)
+        loss = loss + (torch.xlogy(rest, rest) - torch.xlogy(rest, q_rest)).squeeze(1)
+        ratio = torch.where(rest > 0, rest / q_rest, 0.0)
+        grad = q - p - (1 - on) * q * ratio
+        size = q + p + (1 - on) * q * (ratio + 1 / q_rest)
+    loss, grad, size = loss * (1 - a) * temperature**2, grad * (1 - a) * temperature, size * (1 - a) * temperature
+    if a:
+        hard = z.softmax(-1)
+        one = torch.zeros_like(z).scatter_(1, labels.clamp(min=0).long()[:, None], 1.0)
+        loss = loss - a * (z.log_softmax(-1) * one).sum(1)
+        grad, size = grad + a * (hard - one), size + a * (hard + one)
+    if labels is not None:
+        counted = labels != ignore
+        loss, grad = torch.where(counted, loss, 0.0), grad * counted[:, None]
+    return loss, grad, size
+
+
+def lists(z, k, seed, noise=0.5):
+    t = z.float() + made(z.shape, torch.float, seed, noise)
+    top = t.to(z.dtype).topk(k)
+    return top.indices.int(), top.values, t.to(z.dtype)
+
+
+def close(got, want, size, what):
+    dtype = got.dtype
+    allowed = (HALF_ULP[dtype] * want.abs() + SLACK * size + TINY[dtype]) * (1 + 2.0**-10)
+    off = (got.double() - want).abs()
+    bad = ~(off <= allowed)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, by up to {float((off / allowed).nan_to_num(9e9).max()):.3g} times the allowed"
+
+
+CASES = [  # rows, vocab, k, rest, label weight, temperature, labels
+    (1, 1, 1, False, 0.0, 1.0, False), (4, 9, 3, True, 0.0, 1.0, False), (7, 100, 8, False, 0.3, 2.0, True), (5, 1003, 32, True, 0.5, 4.0, True),
+    (3, 2048, 1, True, 0.0, 0.7, True), (6, 8192, 8, False, 0.0, 1.0, True), (3, 16385, 64, True, 1.0, 2.0, True), (2, 30522, 1024, False, 0.0, 1.0, False),
+    (3, 50257, 64, True, 0.25, 2.0, True), (2, 140001, 100, True, 0.25, 1.0, True), (9, 333, 300, False, 0.9, 1.0, True),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,k,rest,a,temperature,labelled", CASES)
+def test_loss_and_gradient(rows, vocab, k, rest, a, temperature, labelled, dtype):
+    z = made((rows, vocab), dtype, vocab)
+    ids, values, t = lists(z, k, vocab + 1)
+    lse = (t.float() / temperature).logsumexp(-1) if rest else None
+    if not rest and k > 1:
+        ids[0, k // 2 :] = -1  # a short list
+    labels = None
+    if labelled:
+        labels = torch.randint(vocab, (rows,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+        labels[0] = int(ids[0, 0])  # on the list
+        labels[-1] = -100
+    loss, grad, size = reference(z, ids, values, lse, labels, a, temperature)
+    count = rows if labels is None else max(1, int((labels != -100).sum()))
+    options = dict(teacher_lse=lse, labels=labels, label_weight=a, temperature=temperature)
+    spread = 2.0**-16 * (1 + float(loss.abs().max())) * max(1.0, temperature**2)
+    got = ps.distill_loss(z, ids, values, reduction="none", **options)
+    assert got.dtype == torch.float and got.shape == (rows,) and ((got.double() - loss).abs() <= spread).all()
+    leaf = z.detach().requires_grad_()
+    scale = torch.tensor(2.0**10, device="cuda")
+    upstream = made((rows,), torch.float, 4, 100.0)
+    (g,) = torch.autograd.grad(ps.distill_loss(leaf, ids, values, reduction="none", **options), leaf, upstream)
+    close(g, grad * upstream.double()[:, None], size * upstream.double().abs()[:, None], "each row")
+    first = None
+    for ahead in (None, scale, 2.0**10, 7.0, scale.double(), torch.tensor(math.nan, device="cuda")):
+        for reduction, divisor in (("mean", count), ("sum", 1)):
+            one = ps.distill_loss(leaf, ids, values, reduction=reduction, grad_scale=ahead, **options)
+            assert one.shape == () and abs(float(one.detach()) * divisor - float(loss.sum())) <= spread * rows
+            (g,) = torch.autograd.grad(one, leaf, scale)
+            close(g, grad * (1024.0 / divisor), size * (1024.0 / divisor), f"{reduction}, {ahead}")
+
+
+def test_gradient_against_differences():
+    z = made((3, 50), torch.float, 1, 1.0).requires_grad_()
+    ids, values, t = lists(z.detach(), 6, 2)
+    lse = (t / 2).logsumexp(-1)
+    labels = torch.tensor([4, -100, 49], device="cuda")
+    options = dict(teacher_lse=lse, labels=labels, label_weight=0.3, temperature=2.0, reduction="none")
+    weight = torch.tensor([1.0, 2.0, -1.5], device="cuda")
+    (g,) = torch.autograd.grad(ps.distill_loss(z, ids, values, **options), z, weight)
+    v = made(z.shape, torch.float, 3, 1.0)
+    h = 2.0**-6
+    with torch.no_grad():
+        up, down = ((ps.distill_loss(z + s * h * v, ids, values, **options).double() * weight.double()).sum() for s in (1, -1))
+    # the outputs' rounding, 2**-22 / 2**-6, and the third derivative's h**2 / 6 of the size
+    assert abs(float(up - down) / (2 * h) - float((g.double() * v.double()).sum())) <= 1e-3 * float(g.norm() * v.norm())
+
+
+def test_rows_that_count_for_nothing():
+    z = made((4, 600), torch.half, 1).requires_grad_()
+    ids, values, t = lists(z.detach(), 8, 2)
+    labels = torch.full((4,), -100, device="cuda")
+    for ahead in (None, 8.0):
+        loss = ps.distill_loss(z, ids, values, labels=labels, label_weight=0.5, grad_scale=ahead)
+        (g,) = torch.autograd.grad(loss, z, torch.tensor(8.0, device="cuda"))
+        assert float(loss.detach()) == 0.0 and (g == 0).all()
+    labels = torch.tensor([-1, 3, -1, -1], device="cuda", dtype=torch.int32)  # another mark, another type
+    want = ps.distill_loss(z[1:2], ids[1:2], values[1:2], labels=labels[1:2])
+    assert torch.equal(ps.distill_loss(z, ids, values, labels=labels, ignore_index=-1), want)
+    # what an ignored row holds does not matter
+    dirty = z.detach().clone()
+    dirty[0], dirty[2] = math.nan, math.inf
+    assert torch.equal(ps.distill_loss(dirty, ids, values, labels=labels, ignore_index=-1), want)
+
+
+def test_lists_that_are_empty_or_hold_everything():
+    z = made((3, 40), torch.float, 1).requires_grad_()
+    ids, values, t = lists(z.detach(), 40, 2)
+    lse = t.logsumexp(-1)
+    none = torch.full_like(ids, -1)
+    for given in (None, lse):
+        loss = ps.distill_loss(z, none, values, teacher_lse=given, reduction="none")
+        (g,) = torch.autograd.grad(loss.sum(), z)
+        assert loss.abs().max() <= 2.0**-20 and g.abs().max() <= 2.0**-20
+    loss, grad, size = reference(z.detach(), ids, values, None, None, 0.0, 1.0)
+    got = ps.distill_loss(z, ids, values, reduction="none")
+    (g,) = torch.autograd.grad(got.sum(), z)
+    assert (got.double() - loss).abs().max() <= 2.0**-16 * (1 + float(loss.max()))
+    close(g, grad, size, "the whole vocabulary")
+
+
+def test_masked_logits():
+    """Tokens that the student may not give: no gradient, and no loss unless the teacher gives them mass."""
+    z = made((2, 3000), torch.half, 1)
+    ids, values, t = lists(z, 16, 2)
+    mask = torch.ones(3000, dtype=torch.bool, device="cuda")
+    mask[:100] = False
+    mask[ids.long().view(-1)] = False
+    z[:, mask] = -math.inf
+    lse = t.float().logsumexp(-1)
+    loss, grad, size = reference(z, ids, values, lse, None, 0.0, 1.0)
+    leaf = z.requires_grad_()
+    got = ps.distill_loss(leaf, ids, values, teacher_lse=lse, reduction="none")
+    (g,) = torch.autograd.grad(got, leaf, torch.full((2,), 64.0, device="cuda"))
+    assert ((got.double() - loss).abs() <= 2.0**-16 * (1 + loss.abs())).all()
+    close(g, grad * 64, size * 64, "gradient")
+    assert (g[:, mask] == 0).all()
+    z = z.detach()
+    z[0, int(ids[0, 0])] = -math.inf
+    got = ps.distill_loss(z, ids, values, reduction="none")
+    assert got[0] == math.inf and got[1].isfinite()
+
+
+def test_wrong_ids_and_labels_show():
+    z = made((5, 700), torch.half, 1).requires_grad_()
+    ids, values, t = lists(z.detach(), 8, 2)
+    labels = torch.tensor([1, 2, 3, 4, 5], device="cuda")
+    ids[0, 3] = 700
+    ids[1, 5] = ids[1, 2]
+    labels[2] = 700
+    labels[3] = -7
+    for ahead in (None, 4.0):
+        loss = ps.distill_loss(z, ids, values, labels=labels, label_weight=0.5, reduction="none" if ahead is None else "sum", grad_scale=ahead)
+        (g,) = torch.autograd.grad(loss, z, torch.full(loss.shape, 4.0, device="cuda"))
+        assert g[:4].isnan().all() and g[4].isfinite().all()
+        if ahead is None:
+            assert loss[:4].isnan().all() and loss[4].isfinite()
+    big = ids.long()
+    big[0, 3] = 2**40  # beyond 32 bits too
+    assert ps.distill_loss(z.detach(), big, values, reduction="none")[0].isnan()
+
+
+def test_a_second_backward_and_a_changed_scale():
+    """The gradient that forward made is given away once, and only at the factor it was made with."""
+    z = made((5, 900), torch.half, 1).requires_grad_()
+    ids, values, t = lists(z.detach(), 8, 2)
+    scale = torch.tensor(256.0, device="cuda")
+    (want,) = torch.autograd.grad(ps.distill_loss(z, ids, values), z, scale)
+    loss = ps.distill_loss(z, ids, values, grad_scale=scale)
+    (a,) = torch.autograd.grad(loss, z, scale, retain_graph=True)
+    a.zero_()  # its owner may write to it
+    (b,) = torch.autograd.grad(loss, z, scale)
+    assert torch.equal(b, want)
+    loss = ps.distill_loss(z, ids, values, grad_scale=scale)
+    scale.mul_(0.5)  # the tensor that was given changes before backward
+    (c,) = torch.autograd.grad(loss, z, scale)
+    (want,) = torch.autograd.grad(ps.distill_loss(z, ids, values), z, scale)
+    assert torch.equal(c, want)
+
+
+def test_strides_and_dimensions_and_the_same_bits_again():
+    """Rows that start elsewhere are summed in another order; the same rows in the same place are not."""
+    whole = made((2, 3, 1100), torch.bfloat16, 1)
+    z = whole[..., 7:1010]
+    ids, values, t = lists(z.reshape(6, -1), 16, 2)
+    lse = t.float().logsumexp(-1)
+    labels = torch.arange(6, device="cuda")
+    loss, grad, size = reference(z.reshape(6, -1), ids, values, lse, labels, 0.5, 1.0)
+    wide_ids, wide_values = torch.cat([ids.long()] * 2, 1)[:, :16], torch.cat([values, values], 1)[:, 16:]
+    first = None
+    for _ in range(3):
+        leaf = z.detach().requires_grad_()
+        got = ps.distill_loss(leaf, wide_ids.unflatten(0, (2, 3)), wide_values.unflatten(0, (2, 3)), lse.view(2, 3), labels.view(2, 3).int(),
+                              label_weight=0.5, grad_scale=8.0)
+        (g,) = torch.autograd.grad(got, leaf, torch.tensor(8.0, device="cuda"))
+        assert abs(float(got.detach()) - float(loss.mean())) <= 2.0**-16 * (1 + float(loss.max()))
+        close(g.view(6, -1), grad * (8 / 6), size * (8 / 6), "gradient")
+        first = first or (got, g)
+        assert torch.equal(got, first[0]) and torch.equal(g, first[1])
+
+
+def test_no_rows():
+    z = torch.empty(0, 50, device="cuda", requires_grad=True)
+    ids, values = torch.empty(0, 4, dtype=torch.int32, device="cuda"), torch.empty(0, 4, device="cuda")
+    loss = ps.distill_loss(z, ids, values)
+    (g,) = torch.autograd.grad(loss, z)
+    assert float(loss.detach()) == 0.0 and g.shape == (0, 50)
+    assert ps.distill_loss(z, ids, values, reduction="none").shape == (0,)
+
+
+def test_on_another_stream_and_in_a_graph():
+    z = made((16, 5000), torch.half, 1).requires_grad_()
+    ids, values, t = lists(z.detach(), 8, 2)
+    labels = torch.arange(16, device="cuda")
+    labels[3] = -100
+    scale = torch.tensor(64.0, device="cuda")
+
+    def both():
+        loss = ps.distill_loss(z, ids, values, labels=labels, label_weight=0.5, grad_scale=scale)
+        return loss, torch.autograd.grad(loss, z, scale)[0]
+
+    want = both()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = both()
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_in_a_graph():
+    """Without autograd: a backward pass in a capture waits for the streams that its leaves were made on."""
+    z = made((16, 5000), torch.half, 1)
+    ids, values, t = lists(z, 8, 2)
+    labels = torch.arange(16, device="cuda")
+    labels[3] = -100
+
+    def run():
+        return (ps.distill_loss(z, ids, values, labels=labels, label_weight=0.5), *ps.top_logits(z, 20, 2.0))
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for n in range(3):
+        z.copy_(made(z.shape, torch.half, 40 + n))
+        labels[n + 4] = -100
+        graph.replay()
+        want = run()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals():
+    z = made((4, 100), torch.half, 1)
+    ids, values, t = lists(z, 8, 2)
+    lse, labels = t.float().logsumexp(-1), torch.zeros(4, dtype=torch.int64, device="cuda")
+    for error, call in [
+        (RuntimeError, lambda: ps.top_logits(z.cpu(), 3)),
+        (TypeError, lambda: ps.top_logits(z.double(), 3)),
+        (ValueError, lambda: ps.top_logits(z, 0)),
+        (ValueError, lambda: ps.top_logits(z, 101)),
+        (ValueError, lambda: ps.top_logits(made((1, 5000), torch.half, 1), 1025)),
+        (ValueError, lambda: ps.top_logits(z, 2.0)),
+        (ValueError, lambda: ps.top_logits(z, 3, temperature=0.0)),
+        (ValueError, lambda: ps.top_logits(z, 3, temperature=math.inf)),
+        (ValueError, lambda: ps.top_logits(z[:, :0], 1)),
+        (RuntimeError, lambda: ps.distill_loss(z.cpu(), ids, values)),
+        (RuntimeError, lambda: ps.distill_loss(z, ids.cpu(), values)),
+        (RuntimeError, lambda: ps.distill_loss(z, ids, values, labels=labels.cpu())),
+        (TypeError, lambda: ps.distill_loss(z, ids.float(), values)),
+        (TypeError, lambda: ps.distill_loss(z, ids, values.double())),
+        (TypeError, lambda: ps.distill_loss(z, ids, values, lse.half())),
+        (TypeError, lambda: ps.distill_loss(z, ids, values, labels=labels.float())),
+        (ValueError, lambda: ps.distill_loss(z, ids[:3], values)),
+        (ValueError, lambda: ps.distill_loss(z, ids, values[:, :7])),
+        (ValueError, lambda: ps.distill_loss(z, ids[:, :0], values[:, :0])),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, lse[:3])),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, labels=labels[:3])),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, label_weight=0.5)),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, labels=labels, label_weight=1.5)),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, temperature=-1.0)),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, reduction="both")),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, reduction="none", grad_scale=2.0)),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, grad_scale=torch.ones(2, device="cuda"))),
+        (ValueError, lambda: ps.distill_loss(z, ids, values, grad_scale=torch.ones(1))),
+    ]:
+        with pytest.raises(error):
+            call()
