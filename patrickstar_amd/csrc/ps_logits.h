@@ -10,11 +10,33 @@
 
 namespace {
 
+// (of lambdas that the kernels call in several places: left to itself the compiler keeps their captures in memory)
+#define PS_INLINE __attribute__((always_inline))
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Softmaxes are taken as exp2(z c - m c), c = log2(e) / temperature and m the row's largest logit: one fused multiply-add in front of
+// the exponential, whose rounding of m c is the same for the whole row and falls out of every quotient.  Where m c would overflow
+// (a row of the type's lowest value, say), two logits that differ at all differ by 2^-24 m at least, so that the smaller one has no
+// mass, and a smaller factor gives the same softmax.
+__device__ __forceinline__ float row_factor(float m, float c)
+{
+    const float size = fabsf(m);
+    return size * c < 1e37f || size == __builtin_inff() ? c : 1e36f / size;
+}
+
 // ---------------------------------------------------------------------------------------------------- a row and its parts
+
+typedef uint32_t raw_t __attribute__((ext_vector_type(4)));  // a vector of a row as it lies in memory
+
+template <typename T>
+struct RowVec {
+    typedef T type __attribute__((ext_vector_type(16 / sizeof(T))));
+    // for rows of the gradient, which may start at any element
+    typedef type __attribute__((aligned(sizeof(T)))) loose;
+};
 
 // The elements of a row: up to VE - 1 in front of the first 16-byte boundary, whole vectors, up to VE - 1 behind the last one.  The
 // ones at the ends are a thread's own each ("lone").
@@ -31,6 +53,17 @@ struct RowShape {
         vectors = (v - head) / VE;
     }
     __device__ __forceinline__ int element_of(int vector) const { return head + vector * VE; }
+    // (a 32-bit offset from an address that is the same for the whole wave: no 64-bit address in registers)
+    __device__ __forceinline__ raw_t vector_at(int vector) const
+    {
+        return *global(reinterpret_cast<const raw_t*>(reinterpret_cast<const char*>(row + head) + (uint32_t)vector * 16u));
+    }
+    // the same vector of another row with this shape, which may start at any element
+    __device__ __forceinline__ void store(T* other, int vector, typename RowVec<T>::type v) const
+    {
+        char* at = reinterpret_cast<char*>(other + head) + (uint32_t)vector * 16u;
+        *(__attribute__((address_space(1))) typename RowVec<T>::loose*)(at) = v;
+    }
     // place of a thread's lone element, or -1
     __device__ __forceinline__ int lone_of(int thread) const
     {
@@ -40,80 +73,108 @@ struct RowShape {
     }
 };
 
+// The thread's number, such that what is computed from it is not kept in registers from one use of the row to the next.
+__device__ __forceinline__ int fresh_thread()
+{
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
+// The largest of the elements given.  NaN is passed over: the sums behind it find it.  (Written as instructions: the compiler puts
+// a canonicalization of every operand in front of its own maximum, which triples the work.)
 template <typename T>
-struct RowVec {
-    typedef T type __attribute__((ext_vector_type(16 / sizeof(T))));
-    // for rows of the gradient, which may start at any element
-    typedef type __attribute__((aligned(sizeof(T)))) loose;
+struct Largest {
+    float top = -__builtin_inff();
+
+    __device__ __forceinline__ void add(raw_t v)
+    {
+        if constexpr (sizeof(T) == 4) {
+            asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top) : "v"(v[0]), "v"(v[1]));
+            asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top) : "v"(v[2]), "v"(v[3]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top) : "v"(v[i] << 16), "v"(v[i] & 0xFFFF0000u));
+        }
+    }
+    __device__ __forceinline__ void add(T x) { top = fmaxf(top, to_float<T>(x)); }
+    __device__ __forceinline__ float get() const { return top; }
+};
+template <>
+struct Largest<half_t> {
+    uint32_t two = 0xFC00FC00u;  // -inf, -inf
+    float top = -__builtin_inff();
+
+    __device__ __forceinline__ void add(raw_t v)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("v_pk_max_f16 %0, %0, %1" : "+v"(two) : "v"(v[i]));
+    }
+    __device__ __forceinline__ void add(half_t x) { top = fmaxf(top, (float)x); }
+    __device__ __forceinline__ float get() const
+    {
+        typedef half_t half2 __attribute__((ext_vector_type(2)));
+        const half2 h = __builtin_bit_cast(half2, two);
+        return fmaxf(top, fmaxf((float)h[0], (float)h[1]));
+    }
 };
 
-template <typename T>
-__device__ __forceinline__ void store_loose(T* p, typename RowVec<T>::type v)
-{
-    *(__attribute__((address_space(1))) typename RowVec<T>::loose*)(p) = v;
-}
-
-template <typename T>
-__device__ __forceinline__ T lowest();
-template <>
-__device__ __forceinline__ half_t lowest<half_t>()
-{
-    return (half_t)-__builtin_inff();
-}
-template <>
-__device__ __forceinline__ bf16_t lowest<bf16_t>()
-{
-    return (bf16_t)-__builtin_inff();
-}
-template <>
-__device__ __forceinline__ float lowest<float>()
-{
-    return -__builtin_inff();
-}
-
-// Calls f(values, first element, count) for the thread's vectors and its lone element; `keep` holds them between calls if NV > 0.
+// A thread's part of a row: its vectors (in registers if NV > 0) and its lone element.
 template <typename T, int NV, int BLOCK>
 struct RowData {
     typedef typename RowVec<T>::type vec;
     static constexpr int VE = RowShape<T>::VE;
-    vec kept[NV > 0 ? NV : 1];
+    raw_t kept[NV > 0 ? NV : 1];
     T lone;
     int lone_at;
 
     __device__ __forceinline__ void load(const RowShape<T>& s)
     {
         lone_at = s.lone_of(threadIdx.x);
-        if (NV > 0) {
+        lone = (T)0.0f;
+        if (lone_at >= 0) lone = *global(s.row + lone_at);
+        const int thread = fresh_thread();
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int v = i * BLOCK + (int)threadIdx.x;
-                if (v < s.vectors) {
-                    kept[i] = *global(reinterpret_cast<const vec*>(s.row + s.element_of(v)));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) kept[i][e] = lowest<T>();
-                }
-            }
+        for (int i = 0; i < NV; ++i) {
+            const int v = i * BLOCK + thread;
+            if (v < s.vectors) kept[i] = s.vector_at(v);
         }
-        lone = lone_at >= 0 ? *global(s.row + lone_at) : lowest<T>();
     }
-    // f(vec, first element) for every vector of the thread that is there, then g(value, element)
+    // What is made of the vectors in one use (their elements in 32 bits) shall not be kept in registers for the next one.
+    __device__ __forceinline__ void hide()
+    {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(kept[i]));
+    }
+    // f(raw vector, its number) for every vector of the thread, then g(value, element) for its lone one
     template <typename F, typename G>
-    __device__ __forceinline__ void each(const RowShape<T>& s, F f, G g) const
+    __device__ __forceinline__ void each_raw(const RowShape<T>& s, F f, G g) const
     {
         if (NV > 0) {
+            const int thread = fresh_thread();
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int v = i * BLOCK + (int)threadIdx.x;
-                if (v < s.vectors) f(kept[i], s.element_of(v));
+                const int v = i * BLOCK + thread;
+                if (v < s.vectors) f(kept[i], v);
+                __builtin_amdgcn_sched_barrier(0);  // vectors worked on side by side would take more registers than there are
             }
         } else {
             for (int v = threadIdx.x; v < s.vectors; v += BLOCK) {
-                const vec x = *global(reinterpret_cast<const vec*>(s.row + s.element_of(v)));
-                f(x, s.element_of(v));
+                f(s.vector_at(v), v);
             }
         }
         if (lone_at >= 0) g(lone, lone_at);
+    }
+    template <typename F, typename G>
+    __device__ __forceinline__ void each(const RowShape<T>& s, F f, G g) const
+    {
+        each_raw(s, [&](raw_t x, int v) PS_INLINE { f(__builtin_bit_cast(vec, x), v); }, g);
+    }
+    __device__ __forceinline__ float largest(const RowShape<T>& s) const
+    {
+        Largest<T> top;
+        each_raw(s, [&](raw_t x, int) PS_INLINE { top.add(x); }, [&](T x, int) PS_INLINE { top.add(x); });
+        return top.get();
     }
 };
 
@@ -178,7 +239,7 @@ struct TopArgs {
     void* values;
     int32_t* ids;
     float* lse;
-    int64_t rows, row_stride;
+    int64_t first_row, row_stride;  // first_row: of this launch
     int vocab, k;
     float factor, temperature;  // log2(e) / temperature
 };
@@ -201,144 +262,231 @@ __device__ __forceinline__ float number_of(uint32_t order)
     return x;  // (NaN: 0x7FFFFFFF)
 }
 
-constexpr int kTopCandidates = 2048;
+constexpr int kTopCandidates = 4096;
+constexpr int kBounds = 16;  // that are tried at a time
 
-// 1. A thread's largest element; the k-th largest of these bounds the k-th largest of the row from below (k threads have one at
-//    least as large), and few elements reach it.  2. Those that do go to LDS; there, an element's place is the number of larger ones.
-// Where too many reach the bound (long runs of equal logits), the k-th largest (order, place) is found bit by bit: all are
-// different, so exactly k reach it.
+// 1. Every thread's largest element.  The k-th largest of these bounds the k-th largest of the row from below (k threads have one
+//    at least as large), and few elements reach it: about k of them where k is small against the threads.  Any smaller bound does
+//    too, so the search for it (kBounds at a time, each counted by a wave over all threads' largest) ends where little more than k
+//    threads reach it.
+// 2. Only those threads' vectors hold candidates: they are read again, spread over all threads.
+// 3. A candidate's place is the number of larger ones.
+// Where too many reach the bound (long runs of equal logits), or NaN or infinities are in the row, the k-th largest (order, place)
+// is found bit by bit: all are different, so exactly k reach it.
 template <typename T, int NV, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void top_logits_kernel(TopArgs p)
+__global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
 {
     typedef typename RowVec<T>::type vec;
     constexpr int VE = RowShape<T>::VE;
+    constexpr int kWaves = BLOCK / 64, kPerWave = kBounds / kWaves;  // (BLOCK <= 1024)
+    // low bits of an order that say nothing: the type's own mantissa is shorter than fp32's by so many
+    constexpr int kLow = sizeof(T) == 4 ? 0 : __is_same(T, half_t) ? 13 : 16;
     __shared__ uint64_t found[kTopCandidates];
     __shared__ uint32_t largest[BLOCK];
-    __shared__ uint32_t lds_max[BLOCK / 64];
-    __shared__ float lds_sum[BLOCK / 64];
-    __shared__ int lds_count[2][BLOCK / 64];
-    __shared__ uint32_t bound_at;
-    __shared__ int n_found;
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    __shared__ uint16_t reaching[BLOCK];
+    __shared__ int place_of[BLOCK];
+    __shared__ uint32_t lds_max[kWaves], lds_min[kWaves];
+    __shared__ float lds_sum[kWaves];
+    __shared__ int lds_count[2][kBounds];
+    __shared__ int n_found, n_reaching;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    {
+        const int64_t r = p.first_row + blockIdx.x;
         const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
         const RowShape<T> shape(row, p.vocab);
         RowData<T, NV, BLOCK> data;
         data.load(shape);
-        uint32_t mine = 0;
-        data.each(
-            shape,
-            [&](const vec& v, int) {
-#pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const uint32_t o = order_of(to_float<T>(v[e]));
-                    mine = o > mine ? o : mine;
-                }
-            },
-            [&](T x, int) {
-                const uint32_t o = order_of(to_float<T>(x));
-                mine = o > mine ? o : mine;
-            });
+        const uint32_t mine = order_of(data.largest(shape));  // (of a thread without elements: -inf's)
         largest[threadIdx.x] = mine;
-        if (threadIdx.x == 0) n_found = 0;
-        const float m = number_of(block_max<BLOCK>(mine, lds_max));  // (a barrier: `largest` is there)
-        // the sum of exponentials; NaN wherever a logit is NaN or +inf
+        if (threadIdx.x == 0) n_found = n_reaching = 0;
+        {
+            const uint32_t hi = wave_max(mine), lo = ~wave_max(~mine);
+            if (lane == 0) lds_max[wave] = hi, lds_min[wave] = lo;
+        }
+        __syncthreads();
+        uint32_t most = lds_max[0], least = lds_min[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            most = lds_max[w] > most ? lds_max[w] : most;
+            least = lds_min[w] < least ? lds_min[w] : least;
+        }
+        const float m = number_of(most), c = row_factor(m, p.factor), mc = m * c;
+        // the sum of exponentials; NaN where a logit is NaN or infinite
         float sum = 0.0f;
+        data.hide();
         data.each(
             shape,
-            [&](const vec& v, int) {
+            [&](const vec& v, int) PS_INLINE {
+                float part = 0.0f;
 #pragma unroll
-                for (int e = 0; e < VE; ++e) sum += exp2_fast((to_float<T>(v[e]) - m) * p.factor);
+                for (int e = 0; e < VE; ++e) part += exp2_fast(__builtin_fmaf(to_float<T>(v[e]), c, -mc));
+                sum += part;
             },
-            [&](T x, int) { sum += exp2_fast((to_float<T>(x) - m) * p.factor); });
-        if (threadIdx.x < 64) {
-            // the k-th largest of the threads' largest: the greatest bound that k of them reach, bit by bit
-            uint32_t bound = 0;
-            if (p.k <= BLOCK) {
-                uint32_t all[BLOCK / 64];
+            [&](T x, int) PS_INLINE { sum += exp2_fast(__builtin_fmaf(to_float<T>(x), c, -mc)); });
+        sum = wave_sum(sum);
+        if (lane == 0) lds_sum[wave] = sum;
+        // the bound: at least k threads reach `bound`, fewer than k `above`
+        uint32_t bound = least, above = most + (most != 0xFFFFFFFFu);
+        int reach = BLOCK;
+        if (p.k <= BLOCK) {
+            const int enough = p.k + p.k / 4 + 8;
+            int turn = 0;
+            while (reach > enough && above - bound > 1) {
+                const uint32_t step = (above - bound) / (kBounds + 1), left = (above - bound) % (kBounds + 1);
+                auto tried = [&](uint32_t i) PS_INLINE { return bound + step * (i + 1) + (left * (i + 1)) / (kBounds + 1); };
+                int n[kPerWave];
 #pragma unroll
-                for (int i = 0; i < BLOCK / 64; ++i) all[i] = largest[i * 64 + threadIdx.x];
-                // bits below the type's own are alike in all numbers of a sign; of fp32 the last ten are left at 0 (a lower bound)
-                constexpr int kLowBit = sizeof(T) == 4 ? 10 : __is_same(T, half_t) ? 13 : 16;
-                for (int bit = 31; bit >= kLowBit; --bit) {
-                    const uint32_t next = bound | 1u << bit;
-                    int n = 0;
+                for (int i = 0; i < kPerWave; ++i) n[i] = 0;
 #pragma unroll
-                    for (int i = 0; i < BLOCK / 64; ++i) n += __popcll(__ballot(all[i] >= next));
-                    if (n >= p.k) bound = next;
+                for (int j = 0; j < kWaves; ++j) {
+                    const uint32_t other = largest[j * 64 + lane];
+#pragma unroll
+                    for (int i = 0; i < kPerWave; ++i) n[i] += __popcll(__ballot(other >= tried(wave * kPerWave + i)));
                 }
+                if (lane == 0) {
+#pragma unroll
+                    for (int i = 0; i < kPerWave; ++i) lds_count[turn][wave * kPerWave + i] = n[i];
+                }
+                __syncthreads();
+                uint32_t new_bound = bound, new_above = above;
+#pragma unroll
+                for (int i = kBounds - 1; i >= 0; --i) {
+                    const int count = lds_count[turn][i];
+                    if (count >= p.k) {
+                        if (new_bound == bound && tried(i) > bound) new_bound = tried(i), reach = count;
+                    } else {
+                        new_above = tried(i);
+                    }
+                }
+                bound = new_bound, above = new_above;
+                turn ^= 1;
             }
-            if (threadIdx.x == 0) bound_at = bound;
         }
-        sum = block_sum<BLOCK>(sum, lds_sum);  // (a barrier: the bound is there)
-        const uint32_t bound = bound_at;
-        if (threadIdx.x == 0) {
-            const bool finite = m - m == 0.0f;  // a row of -inf alone has no mass, one with +inf all of it there; NaN stays
-            const float lse = finite ? m / p.temperature + __builtin_amdgcn_logf(sum) * kLn2 : m;
-            *global(p.lse + r) = lse;
-        }
-        auto keep = [&](uint64_t entry) {
+        __syncthreads();
+        sum = lds_sum[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += lds_sum[w];
+        const bool ordinary = sum - sum == 0.0f;
+        auto keep = [&](uint64_t entry) PS_INLINE {
             const int at = atomicAdd(&n_found, 1);
             if (at < kTopCandidates) found[at] = entry;
         };
-        auto entry_of = [](float x, int at) { return (uint64_t)order_of(x) << 32 | (0xFFFFFFFFu - (uint32_t)at); };
-        if (mine >= bound && mine != 0) {
-            data.each(
-                shape,
-                [&](const vec& v, int at) {
+        auto entry_of = [](float x, int at) PS_INLINE { return (uint64_t)(order_of(x) >> kLow) << 32 | (0xFFFFFFFFu - (uint32_t)at); };
+        bool few = ordinary && p.k <= BLOCK && reach <= 2 * p.k + 64;
+        if (few) {
+            const uint64_t reaches = __ballot(mine >= bound);
+            int at = 0;
+            if (lane == 0 && reaches) at = atomicAdd(&n_reaching, __popcll(reaches));
+            at = __shfl(at, 0);
+            if (mine >= bound) reaching[at + __popcll(reaches & ((1ull << lane) - 1))] = (uint16_t)threadIdx.x;
+            __syncthreads();
+            const float limit = number_of(bound);
+            const int each = (shape.vectors + BLOCK - 1) / BLOCK;  // vectors of a thread
+            const int items = n_reaching * (each + 1);
+            for (int i = threadIdx.x; i < items; i += BLOCK) {
+                const int owner = reaching[i / (each + 1)], part = i % (each + 1), v = part * BLOCK + owner;
+                if (part == each) {
+                    const int place = shape.lone_of(owner);
+                    if (place >= 0) {
+                        const float x = to_float<T>(*global(row + place));
+                        if (x >= limit) keep(entry_of(x, place));
+                    }
+                } else if (v < shape.vectors) {
+                    const vec x = __builtin_bit_cast(vec, shape.vector_at(v));
 #pragma unroll
                     for (int e = 0; e < VE; ++e)
-                        if (order_of(to_float<T>(v[e])) >= bound) keep(entry_of(to_float<T>(v[e]), at + e));
-                },
-                [&](T x, int at) {
-                    if (order_of(to_float<T>(x)) >= bound) keep(entry_of(to_float<T>(x), at));
-                });
+                        if (to_float<T>(x[e]) >= limit) keep(entry_of(to_float<T>(x[e]), shape.element_of(v) + e));
+                }
+            }
+            __syncthreads();
+            few = n_found <= kTopCandidates;
         }
-        __syncthreads();
-        int n = n_found;
-        if (n > kTopCandidates) {
-            uint64_t least = 0;
+        if (!few) {
+            // the row is read again for every bit: what it takes is no ordinary row's concern, and it needs no registers
+            RowData<T, 0, BLOCK> again;
+            again.load(shape);
+            __syncthreads();
+            const int place_bits = 32 - __builtin_clz((uint32_t)p.vocab);
+            uint64_t kth = 0;
             int turn = 0;
-            for (int bit = 63; bit >= 0; --bit) {
-                const uint64_t next = least | 1ull << bit;
+            for (int bit = 63 - kLow; bit >= 0; --bit) {
+                const uint64_t next = kth | 1ull << bit;
+                if (bit < 32 && bit >= place_bits) {  // every entry has these
+                    kth = next;
+                    continue;
+                }
                 int count = 0;
-                data.each(
+                again.each(
                     shape,
-                    [&](const vec& v, int at) {
+                    [&](const vec& v, int i) PS_INLINE {
 #pragma unroll
-                        for (int e = 0; e < VE; ++e) count += entry_of(to_float<T>(v[e]), at + e) >= next;
+                        for (int e = 0; e < VE; ++e) count += entry_of(to_float<T>(v[e]), shape.element_of(i) + e) >= next;
                     },
-                    [&](T x, int at) { count += entry_of(to_float<T>(x), at) >= next; });
+                    [&](T x, int at) PS_INLINE { count += entry_of(to_float<T>(x), at) >= next; });
                 count = block_sum<BLOCK>(count, lds_count[turn]);
                 turn ^= 1;
-                if (count >= p.k) least = next;
+                if (count >= p.k) kth = next;
                 if (count == p.k) break;
             }
             if (threadIdx.x == 0) n_found = 0;
             __syncthreads();
-            data.each(
+            again.each(
                 shape,
-                [&](const vec& v, int at) {
+                [&](const vec& v, int i) PS_INLINE {
 #pragma unroll
-                    for (int e = 0; e < VE; ++e)
-                        if (entry_of(to_float<T>(v[e]), at + e) >= least) keep(entry_of(to_float<T>(v[e]), at + e));
+                    for (int e = 0; e < VE; ++e) {
+                        const uint64_t entry = entry_of(to_float<T>(v[e]), shape.element_of(i) + e);
+                        if (entry >= kth) keep(entry);
+                    }
                 },
-                [&](T x, int at) {
-                    if (entry_of(to_float<T>(x), at) >= least) keep(entry_of(to_float<T>(x), at));
+                [&](T x, int at) PS_INLINE {
+                    if (entry_of(to_float<T>(x), at) >= kth) keep(entry_of(to_float<T>(x), at));
                 });
             __syncthreads();
-            n = n_found;
         }
-        for (int i = threadIdx.x; i < n; i += BLOCK) {
-            const uint64_t mine_entry = found[i];
-            int place = 0;
-            for (int j = 0; j < n; ++j) place += found[j] > mine_entry;
-            if (place < p.k) {
-                const uint32_t at = 0xFFFFFFFFu - (uint32_t)mine_entry;
+        const int n = n_found;
+        if (threadIdx.x == 0) {
+            float lse = c == p.factor ? (mc + __builtin_amdgcn_logf(sum)) * kLn2 : m / p.temperature;
+            if (!ordinary) {  // the row's largest, NaN being larger than everything: a row of -inf alone has no mass
+                uint64_t first = 0;
+                for (int i = 0; i < n; ++i) first = found[i] > first ? found[i] : first;
+                const uint32_t order = (uint32_t)(first >> 32) << kLow;
+                lse = number_of(order & 0x80000000u ? order : order | ((1u << kLow) - 1));
+                if (order == 0xFFFFFFFFu >> kLow << kLow) lse = __builtin_nanf("");
+            }
+            *global(p.lse + r) = lse;
+        }
+        if (n <= BLOCK) {
+            int span = 64;
+            while (span < n) span *= 2;
+            const int slices = BLOCK / span, mine_at = threadIdx.x & (span - 1), slice = threadIdx.x / span;
+            place_of[threadIdx.x] = 0;
+            __syncthreads();
+            const uint64_t entry = mine_at < n ? found[mine_at] : 0;
+            if (mine_at < n) {
+                int count = 0;
+                for (int j = slice; j < n; j += slices) count += found[j] > entry;
+                if (count) atomicAdd(&place_of[mine_at], count);
+            }
+            __syncthreads();
+            const int place = place_of[mine_at];
+            if (slice == 0 && mine_at < n && place < p.k) {
+                const uint32_t at = 0xFFFFFFFFu - (uint32_t)entry;
                 *global(p.ids + r * p.k + place) = (int32_t)at;
                 *global(static_cast<T*>(p.values) + r * p.k + place) = *global(row + at);
             }
+        } else {
+            for (int i = threadIdx.x; i < n; i += BLOCK) {
+                const uint64_t entry = found[i];
+                int place = 0;
+                for (int j = 0; j < n; ++j) place += found[j] > entry;
+                if (place < p.k) {
+                    const uint32_t at = 0xFFFFFFFFu - (uint32_t)entry;
+                    *global(p.ids + r * p.k + place) = (int32_t)at;
+                    *global(static_cast<T*>(p.values) + r * p.k + place) = *global(row + at);
+                }
+            }
         }
-        __syncthreads();  // before the next row's candidates
     }
 }
 
@@ -356,7 +504,7 @@ struct DistillArgs {
     void* grad;
     const float* upstream;
     float* upstream_used;
-    int64_t rows, row_stride, ids_stride, values_stride, upstream_stride;
+    int64_t rows, first_row, row_stride, ids_stride, values_stride, upstream_stride;  // first_row: of this launch
     int64_t ignore_index;
     int vocab, k;
     int values_dtype;
@@ -381,6 +529,41 @@ struct RowStats {
     float inv_s;   // 1 / sum of exp((z - m) / temperature)
     float coef;    // a softmax's share in the gradient off the list: 1 - rest / q_rest, or the list's mass
     float inv_s1;  // 1 / sum of exp(z - m)
+};
+
+// How the two softmaxes of a row, at the temperature and at 1, come from one another: at temperature 1, or if only one of the two is
+// wanted, there is one; at 2 the second's exponential is the first's square; else each has its own.
+enum { kOne, kSquare, kTwo };
+
+// Calls f(Int<how>) for the row's way.
+template <typename F>
+__device__ __forceinline__ auto with_softmaxes(const DistillArgs& p, F f)
+{
+    const bool both = p.label_weight != 0.0f && p.label_weight != 1.0f;
+    if (!both || p.temperature == 1.0f) return f(Int<kOne>());
+    if (p.temperature == 2.0f) return f(Int<kSquare>());
+    return f(Int<kTwo>());
+}
+
+// The exponentials of a logit: e at the temperature (at 1 if there is no other), e1 at 1.
+struct Exponents {
+    float c, mc, c1, mc1;
+
+    __device__ __forceinline__ Exponents(const DistillArgs& p, float m)
+    {
+        c = row_factor(m, p.label_weight == 1.0f ? kLog2e : kLog2e / p.temperature);
+        mc = m * c;
+        c1 = row_factor(m, kLog2e);
+        mc1 = m * c1;
+    }
+    template <int HOW>
+    __device__ __forceinline__ void of(float z, float& e, float& e1) const
+    {
+        e = exp2_fast(__builtin_fmaf(z, c, -mc));
+        if (HOW == kOne) e1 = e;
+        if (HOW == kSquare) e1 = e * e;
+        if (HOW == kTwo) e1 = exp2_fast(__builtin_fmaf(z, c1, -mc1));
+    }
 };
 
 // The teacher's list in LDS: ids, probabilities.  Returns through `mass` their sum (every thread).
@@ -417,71 +600,57 @@ __device__ __forceinline__ void load_list(const DistillArgs& p, int64_t r, int* 
 
 // The row's gradient, from registers or memory: list entries and label after everything else, over it.
 template <typename T, int NV, int BLOCK>
-__device__ __forceinline__ void write_gradient(const DistillArgs& p, int64_t r, const RowShape<T>& shape, const RowData<T, NV, BLOCK>& data,
+__device__ __forceinline__ void write_gradient(const DistillArgs& p, int64_t r, const RowShape<T>& shape, RowData<T, NV, BLOCK>& data,
                                                const RowStats& s, float factor, const int* ids, const float* prob, int64_t label)
 {
     typedef typename RowVec<T>::type vec;
     constexpr int VE = RowShape<T>::VE;
     T* out = static_cast<T*>(p.grad) + r * (int64_t)p.vocab;
-    const float c = kLog2e / p.temperature;
-    const float soft = factor * (1.0f - p.label_weight) * p.temperature * s.inv_s;
-    const float hard = factor * p.label_weight * s.inv_s1;
-    const float off = soft * s.coef;
     const bool soft_there = p.label_weight != 1.0f, hard_there = p.label_weight != 0.0f;
-    const bool both = soft_there && hard_there;
-    const float c1 = soft_there ? c : kLog2e, a1 = soft_there ? off : hard;
-    if (both) {
+    const float soft = soft_there ? factor * (1.0f - p.label_weight) * p.temperature * s.inv_s : 0.0f;
+    const float hard = hard_there ? factor * p.label_weight * s.inv_s1 : 0.0f;
+    const float off = soft_there ? soft * s.coef : 0.0f;
+    const Exponents exponents(p, s.m);
+    data.hide();
+    with_softmaxes(p, [&](auto how) PS_INLINE {
+        const float share = how() == kOne ? off + hard : off;
+        auto gradient = [&](float z) PS_INLINE {
+            float e, e1;
+            exponents.of<how()>(z, e, e1);
+            return __builtin_fmaf(e, share, how() == kOne ? 0.0f : e1 * hard);
+        };
         data.each(
             shape,
-            [&](const vec& v, int at) {
+            [&](const vec& v, int i) PS_INLINE {
                 vec g;
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const float d = to_float<T>(v[e]) - s.m;
-                    g[e] = from_float<T>(__builtin_fmaf(exp2_fast(d * c), off, exp2_fast(d * kLog2e) * hard));
-                }
-                store_loose<T>(out + at, g);
+                for (int e = 0; e < VE; ++e) g[e] = from_float<T>(gradient(to_float<T>(v[e])));
+                shape.store(out, i, g);
             },
-            [&](T x, int at) {
-                const float d = to_float<T>(x) - s.m;
-                *global(out + at) = from_float<T>(__builtin_fmaf(exp2_fast(d * c), off, exp2_fast(d * kLog2e) * hard));
-            });
-    } else {
-        data.each(
-            shape,
-            [&](const vec& v, int at) {
-                vec g;
-#pragma unroll
-                for (int e = 0; e < VE; ++e) g[e] = from_float<T>(exp2_fast((to_float<T>(v[e]) - s.m) * c1) * a1);
-                store_loose<T>(out + at, g);
-            },
-            [&](T x, int at) { *global(out + at) = from_float<T>(exp2_fast((to_float<T>(x) - s.m) * c1) * a1); });
-    }
-    __syncthreads();
-    const float mass_factor = p.teacher_lse != nullptr ? 1.0f : s.coef;
-    const float given = factor * (1.0f - p.label_weight) * p.temperature;
-    if (soft_there) {
-        for (int i = threadIdx.x; i < p.k; i += BLOCK) {
-            const int id = ids[i];
-            if (id < 0) continue;
-            const float d = to_float<T>(*global(shape.row + id)) - s.m;
-            float g = exp2_fast(d * c) * soft * mass_factor - given * prob[i];
-            if (hard_there) g += exp2_fast(d * kLog2e) * hard - (id == label ? factor * p.label_weight : 0.0f);
-            *global(out + id) = from_float<T>(g);
+            [&](T x, int at) PS_INLINE { *global(out + at) = from_float<T>(gradient(to_float<T>(x))); });
+        __syncthreads();
+        const float mass_share = p.teacher_lse != nullptr ? soft : off;
+        const float given = factor * (1.0f - p.label_weight) * p.temperature;
+        if (soft_there) {
+            for (int i = threadIdx.x; i < p.k; i += BLOCK) {
+                const int id = ids[i];
+                if (id < 0) continue;
+                float e, e1;
+                exponents.of<how()>(to_float<T>(*global(shape.row + id)), e, e1);
+                float g = __builtin_fmaf(e, mass_share, -given * prob[i]);
+                if (hard_there) g += e1 * hard - (id == label ? factor * p.label_weight : 0.0f);
+                *global(out + id) = from_float<T>(g);
+            }
         }
-    }
-    if (hard_there) {
-        // the label, unless it is on the list: the thread of its entry has written it
-        bool listed = false;
-        if (soft_there)
-            for (int i = threadIdx.x; i < p.k; i += BLOCK) listed |= ids[i] == label;
-        if (!__syncthreads_or(listed) && threadIdx.x == 0 && label >= 0 && label < p.vocab) {
-            const float d = to_float<T>(*global(shape.row + label)) - s.m;
-            float g = exp2_fast(d * kLog2e) * hard - factor * p.label_weight;
-            if (soft_there) g += exp2_fast(d * c) * off;
-            *global(out + label) = from_float<T>(g);
+        if (hard_there) {
+            // the label, unless it is on the list: the thread of its entry has written it
+            bool listed = false;
+            if (soft_there)
+                for (int i = threadIdx.x; i < p.k; i += BLOCK) listed |= ids[i] == label;
+            if (!__syncthreads_or(listed) && threadIdx.x == 0 && label >= 0 && label < p.vocab)
+                *global(out + label) = from_float<T>(gradient(to_float<T>(*global(shape.row + label))) - factor * p.label_weight);
         }
-    }
+    });
 }
 
 template <typename T, int NV, int BLOCK>
@@ -492,30 +661,91 @@ __device__ __forceinline__ void write_zeros(const DistillArgs& p, int64_t r, con
     vec zero;
 #pragma unroll
     for (int e = 0; e < RowShape<T>::VE; ++e) zero[e] = (T)0.0f;
-    for (int v = threadIdx.x; v < shape.vectors; v += BLOCK) store_loose<T>(out + shape.element_of(v), zero);
+    for (int v = threadIdx.x; v < shape.vectors; v += BLOCK) shape.store(out, v, zero);
     const int lone = shape.lone_of(threadIdx.x);
     if (lone >= 0) *global(out + lone) = (T)0.0f;
 }
 
+// Words of LDS that hold a bit for every token.  The first token's bit is moved so that a vector's bits begin at its own byte or half
+// byte.
+__host__ __device__ constexpr int member_words(int vocab) { return (vocab + 8 + 31) / 32; }
+
+template <typename T>
+struct Members {
+    static constexpr int VE = RowShape<T>::VE;
+    uint32_t* words;
+    int shift;
+
+    __device__ __forceinline__ Members(uint32_t* w, const RowShape<T>& s) : words(w), shift((VE - s.head) & (VE - 1)) {}
+    // whether it was there
+    __device__ __forceinline__ bool add(int id) const
+    {
+        const int bit = id + shift;
+        return atomicOr(&words[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1;
+    }
+    __device__ __forceinline__ bool has(int id) const { return words[(id + shift) >> 5] >> ((id + shift) & 31) & 1; }
+    // the bits of the vector that begins with this element
+    __device__ __forceinline__ uint32_t of_vector(int first) const
+    {
+        const uint32_t bit = (uint32_t)(first + shift);
+        return reinterpret_cast<const uint8_t*>(words)[bit >> 3] >> (bit & 7) & ((1u << VE) - 1);
+    }
+};
+
+struct RowSums {
+    float all, rest, at_1;  // of the exponentials: everything, off the list, at temperature 1
+};
+
+// A thread's part of the row's sums.
+template <int HOW, bool REST, typename T, int NV, int BLOCK>
+__device__ __forceinline__ RowSums add_up(const RowData<T, NV, BLOCK>& data, const RowShape<T>& shape, const Exponents& exponents,
+                                          const Members<T>& members)
+{
+    constexpr int VE = RowShape<T>::VE;
+    float all = 0.0f, rest = 0.0f, at_1 = 0.0f;
+    data.each(
+        shape,
+        [&](const typename RowVec<T>::type& v, int i) PS_INLINE {
+            float part = 0.0f;
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                float e, e1;
+                exponents.of<HOW>(to_float<T>(v[k]), e, e1);
+                part += e;
+                if (HOW != kOne) at_1 += e1;
+            }
+            all += part;
+            if (REST) rest += members.of_vector(shape.element_of(i)) ? 0.0f : part;
+        },
+        [&](T z, int at) PS_INLINE {
+            float e, e1;
+            exponents.of<HOW>(to_float<T>(z), e, e1);
+            all += e;
+            if (HOW != kOne) at_1 += e1;
+            if (REST && !members.has(at)) rest += e;
+        });
+    return {all, rest, HOW == kOne ? all : at_1};
+}
+
 // Dynamic LDS: a bit for every token of the vocabulary (is it on the list?), then the list's ids and probabilities.
 template <typename T, int NV, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void distill_loss_kernel(DistillArgs p)
+__global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
 {
     typedef typename RowVec<T>::type vec;
     constexpr int VE = RowShape<T>::VE;
     extern __shared__ uint32_t dynamic[];
     __shared__ float lds[6][BLOCK / 64];
-    const int words = (p.vocab + 31) / 32;
+    const int words = member_words(p.vocab);
     uint32_t* member = dynamic;
     int* ids = reinterpret_cast<int*>(dynamic + words);
     float* prob = reinterpret_cast<float*>(dynamic + words + p.k);
     const bool rest = p.teacher_lse != nullptr;
     const bool soft = p.label_weight != 1.0f, hard = p.label_weight != 0.0f;
-    const float c = kLog2e / p.temperature;
     const float upstream = p.upstream ? *global(p.upstream) : p.upstream_value;
-    if (p.upstream_used && blockIdx.x == 0 && threadIdx.x == 0) *global(p.upstream_used) = upstream;
+    if (p.upstream_used && p.first_row + blockIdx.x == 0 && threadIdx.x == 0) *global(p.upstream_used) = upstream;
     const float inv_count = p.denominator ? 1.0f / *global(p.denominator) : 1.0f;
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    {
+        const int64_t r = p.first_row + blockIdx.x;
         const RowShape<T> shape(static_cast<const T*>(p.logits) + r * p.row_stride, p.vocab);
         int64_t label = -1;
         bool wrong = false;
@@ -528,7 +758,7 @@ __global__ __launch_bounds__(BLOCK) void distill_loss_kernel(DistillArgs p)
                         for (int i = 0; i < 4; ++i) *global(p.stats + 4 * r + i) = 0.0f;
                 }
                 if (p.grad) write_zeros<T, NV, BLOCK>(p, r, shape);
-                continue;
+                return;
             }
             if (hard) wrong = label < 0 || label >= p.vocab;
         }
@@ -537,64 +767,44 @@ __global__ __launch_bounds__(BLOCK) void distill_loss_kernel(DistillArgs p)
         for (int i = threadIdx.x; i < words; i += BLOCK) member[i] = 0;
         float mass;
         load_list<BLOCK>(p, r, ids, prob, lds[0], lds[1], mass);
+        const Members<T> members(member, shape);
         for (int i = threadIdx.x; i < p.k; i += BLOCK) {
             const int id = ids[i];
-            if (id >= 0)
-                wrong |= (atomicOr(&member[id >> 5], 1u << (id & 31)) >> (id & 31)) & 1;
-            else
-                wrong |= id == -2;
+            wrong |= id >= 0 ? members.add(id) : id == -2;
         }
-        float m = -__builtin_inff();
-        data.each(
-            shape,
-            [&](const vec& v, int) {
+        const float m = block_max<BLOCK, float>(data.largest(shape), lds[2]);  // (a barrier: the members are there)
+        const Exponents exponents(p, m);
+        data.hide();
+        const RowSums sums = with_softmaxes(p, [&](auto how) PS_INLINE {
+            if (rest && soft) return add_up<how(), true, T, NV, BLOCK>(data, shape, exponents, members);
+            return add_up<how(), false, T, NV, BLOCK>(data, shape, exponents, members);
+        });
+        float sum = sums.all, sum_rest = sums.rest, sum1 = sums.at_1;
+        if (rest && soft) {
+            // what is off the list in vectors that hold a token of it: the thread of the first such token sees to it
+            for (int i = threadIdx.x; i < p.k; i += BLOCK) {
+                const int id = ids[i];
+                if (id < shape.head || id >= shape.element_of(shape.vectors)) continue;
+                const int number = (id - shape.head) / VE, first = shape.element_of(number);
+                const uint32_t bits = members.of_vector(first);
+                if (bits & ((1u << (id - first)) - 1)) continue;
+                const vec v = __builtin_bit_cast(vec, shape.vector_at(number));
 #pragma unroll
-                for (int e = 0; e < VE; ++e) m = fmaxf(m, to_float<T>(v[e]));
-            },
-            [&](T x, int) { m = fmaxf(m, to_float<T>(x)); });
-        m = block_max<BLOCK, float>(m, lds[2]);  // (a barrier: the members are there)
-        float sum = 0.0f, sum_rest = 0.0f, sum1 = 0.0f;
-        const float first = soft ? c : kLog2e;
-        data.each(
-            shape,
-            [&](const vec& v, int at) {
-                float part = 0.0f;
-                float x[VE];
-#pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    x[e] = exp2_fast((to_float<T>(v[e]) - m) * first);
-                    part += x[e];
-                }
-                sum += part;
-                if (rest) {
-                    // the vector's members: VE bits that may lie in two words
-                    const uint32_t lo = member[at >> 5], hi = member[(at + VE - 1) >> 5];
-                    const uint32_t bits = (uint32_t)(((uint64_t)hi << 32 | lo) >> (at & 31)) & ((1u << VE) - 1);
-                    if (bits) {
-                        part = 0.0f;
-#pragma unroll
-                        for (int e = 0; e < VE; ++e) part += bits >> e & 1 ? 0.0f : x[e];
-                    }
-                    sum_rest += part;
-                }
-                if (soft && hard) {
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) sum1 += exp2_fast((to_float<T>(v[e]) - m) * kLog2e);
-                }
-            },
-            [&](T x, int at) {
-                const float e = exp2_fast((to_float<T>(x) - m) * first);
-                sum += e;
-                if (rest && !(member[at >> 5] >> (at & 31) & 1)) sum_rest += e;
-                if (soft && hard) sum1 += exp2_fast((to_float<T>(x) - m) * kLog2e);
-            });
-        // the list's part of the divergence does not need the sums: sum p (log p - z) and sum p
+                for (int e = 0; e < VE; ++e)
+                    sum_rest += bits >> e & 1 ? 0.0f : exp2_fast(__builtin_fmaf(to_float<T>(v[e]), exponents.c, -exponents.mc));
+            }
+        }
+        // the list's part of the divergence: sum p (log p - log q) without q's normaliser, which sum p takes
         float term = 0.0f;
+        const bool usual = exponents.c == kLog2e / p.temperature;
         if (soft) {
             for (int i = threadIdx.x; i < p.k; i += BLOCK) {
                 const float pr = prob[i];
-                if (ids[i] >= 0 && pr != 0.0f)
-                    term = __builtin_fmaf(pr, logf(pr) - (to_float<T>(*global(shape.row + ids[i])) - m) / p.temperature, term);
+                if (ids[i] >= 0 && pr != 0.0f) {
+                    const float z = to_float<T>(*global(shape.row + ids[i]));
+                    const float log_q = usual ? __builtin_fmaf(z, exponents.c, -exponents.mc) * kLn2 : (z - m) / p.temperature;
+                    term = __builtin_fmaf(pr, logf(pr) - log_q, term);
+                }
             }
         }
         sum = wave_sum(sum), sum_rest = wave_sum(sum_rest), sum1 = wave_sum(sum1), term = wave_sum(term);
@@ -613,24 +823,24 @@ __global__ __launch_bounds__(BLOCK) void distill_loss_kernel(DistillArgs p)
             sum1 += lds[3][w];
             term += lds[4][w];
         }
-        if (!soft) sum1 = sum;
         if (wrong) sum = sum1 = __builtin_nanf("");
         RowStats s;
         s.m = m;
-        s.inv_s = soft ? 1.0f / sum : 0.0f;
-        s.inv_s1 = hard ? 1.0f / sum1 : 0.0f;
+        s.inv_s = 1.0f / sum;
+        s.inv_s1 = 1.0f / sum1;
         const float p_rest = fmaxf(1.0f - mass, 0.0f), q_rest = sum_rest * s.inv_s;
         s.coef = rest ? (p_rest == 0.0f ? 1.0f : 1.0f - p_rest / q_rest) : mass;
         if (threadIdx.x == 0) {
             float loss = 0.0f;
             if (soft) {
-                float kl = __builtin_fmaf(mass, logf(sum), term);  // + sum p log s
+                float kl = __builtin_fmaf(mass, logf(sum), term);
                 if (rest && p_rest > 0.0f) kl = __builtin_fmaf(p_rest, logf(p_rest) - logf(q_rest), kl);
                 loss = (1.0f - p.label_weight) * p.temperature * p.temperature * kl;
             }
             if (hard) {
                 const float z = wrong ? m : to_float<T>(*global(shape.row + label));
-                loss = __builtin_fmaf(p.label_weight, logf(sum1) - (z - m), loss);
+                const float log_q = exponents.c1 == kLog2e ? __builtin_fmaf(z, kLog2e, -exponents.mc1) * kLn2 : z - m;
+                loss = __builtin_fmaf(p.label_weight, logf(sum1) - log_q, loss);
             }
             *global(p.row_loss + r) = loss;
             if (p.stats) {
@@ -641,7 +851,6 @@ __global__ __launch_bounds__(BLOCK) void distill_loss_kernel(DistillArgs p)
             }
         }
         if (p.grad) write_gradient<T, NV, BLOCK>(p, r, shape, data, s, upstream * inv_count, ids, prob, label);
-        __syncthreads();  // before the next row's list
     }
 }
 
@@ -655,12 +864,13 @@ __global__ __launch_bounds__(BLOCK) void distill_backward_kernel(DistillArgs p)
     int* ids = reinterpret_cast<int*>(dynamic);
     float* prob = reinterpret_cast<float*>(dynamic + p.k);
     const float inv_count = p.denominator ? 1.0f / *global(p.denominator) : 1.0f;
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    {
+        const int64_t r = p.first_row + blockIdx.x;
         const RowShape<T> shape(static_cast<const T*>(p.logits) + r * p.row_stride, p.vocab);
         const int64_t label = p.labels ? whole_at(p.labels, r, p.labels_64) : -1;
         if (p.labels && label == p.ignore_index) {
             write_zeros<T, 0, BLOCK>(p, r, shape);
-            continue;
+            return;
         }
         RowStats s;
         s.m = *global(p.stats + 4 * r);
@@ -672,7 +882,6 @@ __global__ __launch_bounds__(BLOCK) void distill_backward_kernel(DistillArgs p)
         RowData<T, 0, BLOCK> data;
         data.load(shape);
         write_gradient<T, 0, BLOCK>(p, r, shape, data, s, *global(p.upstream + r * p.upstream_stride) * inv_count, ids, prob, label);
-        __syncthreads();
     }
 }
 

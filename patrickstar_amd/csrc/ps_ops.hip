@@ -31,9 +31,6 @@ void with_type(int dtype, F f)
         f(float());
 }
 
-template <int N>
-using Int = std::integral_constant<int, N>;
-
 // ---------------------------------------------------------------------------------------------------------- rotations
 
 int check_heads(const ps_heads_call* c, bool backward)
@@ -158,25 +155,38 @@ bool wants_weight_grad(const ps_heads_call* c)
 
 // ------------------------------------------------------------------------------------------------------------- logits
 
-// Calls f(vectors a thread keeps, threads): the shortest row that holds the vocabulary; 0 where none does.
+// Calls f(vectors a thread keeps, threads), with at least `threads` of them: the shortest row that holds the vocabulary; 0 where
+// none does.
 template <typename T, typename F>
-void with_row(int vocab, bool wide, F f)
+void with_row(int vocab, int threads, F f)
 {
     const int vectors = vocab / (16 / (int)sizeof(T)) + 1;
-    if (!wide) {
+    if (threads <= 256) {
         if (vectors <= 256) return f(Int<1>(), Int<256>());
         if (vectors <= 512) return f(Int<2>(), Int<256>());
         if (vectors <= 1024) return f(Int<4>(), Int<256>());
         if (vectors <= 2048) return f(Int<8>(), Int<256>());
     }
-    if (vectors <= 2048) return f(Int<2>(), Int<1024>());
+    if (threads <= 512) {
+        if (vectors <= 4096) return f(Int<8>(), Int<512>());
+        if (vectors <= 8192) return f(Int<16>(), Int<512>());
+    }
     if (vectors <= 4096) return f(Int<4>(), Int<1024>());
-    if (vectors <= 8192) return f(Int<8>(), Int<1024>());
     if (vectors <= 16384) return f(Int<16>(), Int<1024>());
     f(Int<0>(), Int<1024>());
 }
 
-unsigned row_blocks(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 21); }
+// Calls launch(first row, workgroups) for all rows: a workgroup each, and no more than a grid takes.
+template <typename F>
+int for_rows(int64_t rows, F launch)
+{
+    constexpr int64_t kMost = 1 << 21;
+    for (int64_t first = 0; first < rows; first += kMost) {
+        launch(first, dim3((unsigned)std::min(rows - first, kMost)));
+        PS_HIP(hipGetLastError());
+    }
+    return 0;
+}
 
 constexpr int64_t kMaxTopVocab = 1 << 30;
 constexpr int64_t kMaxDistillVocab = 400000;  // a bit each in LDS, beside a list
@@ -312,20 +322,20 @@ int ps_top_logits(const ps_top_call* call, ps_stream_t stream)
     a.values = call->values;
     a.ids = call->ids;
     a.lse = call->lse;
-    a.rows = call->rows;
     a.row_stride = call->row_stride;
     a.vocab = (int)call->vocab;
     a.k = call->k;
     a.factor = (float)(1.4426950408889634 / (double)call->temperature);
     a.temperature = call->temperature;
-    with_type(call->dtype, [&](auto t) {
-        typedef decltype(t) T;
-        with_row<T>(a.vocab, a.k > 128, [&](auto nv, auto block) {
-            hipLaunchKernelGGL((top_logits_kernel<T, nv(), block()>), dim3(row_blocks(a.rows)), dim3(block()), 0, static_cast<hipStream_t>(stream), a);
+    return for_rows(call->rows, [&](int64_t first, dim3 grid) {
+        a.first_row = first;
+        with_type(call->dtype, [&](auto t) {
+            typedef decltype(t) T;
+            with_row<T>(a.vocab, a.k <= 128 ? 256 : a.k <= 400 ? 512 : 1024, [&](auto nv, auto block) {
+                hipLaunchKernelGGL((top_logits_kernel<T, nv(), block()>), grid, dim3(block()), 0, static_cast<hipStream_t>(stream), a);
+            });
         });
     });
-    PS_HIP(hipGetLastError());
-    return 0;
 }
 
 int ps_distill_loss(const ps_distill_call* call, ps_stream_t stream)
@@ -337,16 +347,17 @@ int ps_distill_loss(const ps_distill_call* call, ps_stream_t stream)
         hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, st, call->labels, a.labels_64, a.rows, a.ignore_index, call->denominator);
         PS_HIP(hipGetLastError());
     }
-    if (a.rows) {
-        const unsigned lds = 4u * (unsigned)((a.vocab + 31) / 32) + 8u * (unsigned)a.k;
+    const unsigned lds = 4u * (unsigned)member_words(a.vocab) + 8u * (unsigned)a.k;
+    const int rc = for_rows(a.rows, [&](int64_t first, dim3 grid) {
+        a.first_row = first;
         with_type(call->dtype, [&](auto t) {
             typedef decltype(t) T;
-            with_row<T>(a.vocab, false, [&](auto nv, auto block) {
-                hipLaunchKernelGGL((distill_loss_kernel<T, nv(), block()>), dim3(row_blocks(a.rows)), dim3(block()), lds, st, a);
+            with_row<T>(a.vocab, 256, [&](auto nv, auto block) {
+                hipLaunchKernelGGL((distill_loss_kernel<T, nv(), block()>), grid, dim3(block()), lds, st, a);
             });
         });
-        PS_HIP(hipGetLastError());
-    }
+    });
+    if (rc) return rc;
     if (call->loss) {
         hipLaunchKernelGGL(sum_rows_kernel, dim3(1), dim3(1024), 0, st, call->row_loss, a.rows, a.denominator, call->loss);
         PS_HIP(hipGetLastError());
@@ -358,13 +369,13 @@ int ps_distill_loss_backward(const ps_distill_call* call, ps_stream_t stream)
 {
     DistillArgs a;
     if (int rc = distill_args(call, true, a)) return rc;
-    if (a.rows == 0) return 0;
-    with_type(call->dtype, [&](auto t) {
-        typedef decltype(t) T;
-        hipLaunchKernelGGL((distill_backward_kernel<T, 256>), dim3(row_blocks(a.rows)), dim3(256), 8u * (unsigned)a.k, static_cast<hipStream_t>(stream), a);
+    return for_rows(a.rows, [&](int64_t first, dim3 grid) {
+        a.first_row = first;
+        with_type(call->dtype, [&](auto t) {
+            typedef decltype(t) T;
+            hipLaunchKernelGGL((distill_backward_kernel<T, 256>), grid, dim3(256), 8u * (unsigned)a.k, static_cast<hipStream_t>(stream), a);
+        });
     });
-    PS_HIP(hipGetLastError());
-    return 0;
 }
 
 }  // extern "C"

@@ -5,11 +5,15 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace {
 
 typedef _Float16 half_t;
 typedef __bf16 bf16_t;
+
+template <int N>
+using Int = std::integral_constant<int, N>;
 
 // Operands are device memory: said so, the compiler need not use flat accesses.
 template <typename T>
