@@ -15,6 +15,9 @@ namespace {
 
 constexpr int kCus = 256;
 
+// Workgroups of the rotations, which loop over their tokens.
+constexpr uint32_t kForwardBlocks = 16 * kCus, kBackwardBlocks = 4 * kCus;
+
 int size_of(int dtype) { return dtype == PS_F32 ? 4 : 2; }
 
 bool known(int dtype) { return dtype == PS_F16 || dtype == PS_BF16 || dtype == PS_F32; }
@@ -81,24 +84,37 @@ bool fits_vectors(const ps_heads_call* c, int v, bool backward)
 
 struct HeadsShape {
     HeadsArgs a;
-    int v;               // elements of a vector
-    uint32_t waves;      // that the call's tokens take
-    uint32_t splits;     // of a token's heads
+    int v;            // elements of a vector
+    uint32_t blocks;  // of queries and keys together
 };
+
+// A wave's items of queries or keys, and the workgroups that take them.
+void shape_part(const ps_heads_call* c, int which, const HeadsArgs& a, uint32_t most_blocks, HeadsPart& part)
+{
+    part.x = c->x[which];
+    part.grad = c->grad[which];
+    part.out = c->out[which];
+    part.weight = c->weight[which];
+    memcpy(part.x_stride, c->x_stride[which], sizeof(part.x_stride));
+    memcpy(part.grad_stride, c->grad_stride[which], sizeof(part.grad_stride));
+    part.heads = c->heads[which];
+    if (part.heads == 0) return;
+    part.weight_vectors = (uintptr_t)part.weight % 16 == 0;
+    while ((1 << part.slot_shift) < part.heads && part.slot_shift < 6 - a.group_shift) ++part.slot_shift;
+    const int tokens_shift = 6 - a.group_shift - part.slot_shift;
+    const uint32_t waves = (uint32_t)(((uint64_t)a.all_tokens + (1u << tokens_shift) - 1) >> tokens_shift);
+    // few tokens: a token's heads are spread over more waves, each of which makes the token's angles for itself
+    while ((part.heads >> (part.slot_shift + part.split_shift)) > 1 && ((uint64_t)waves << part.split_shift) < 8 * kCus) ++part.split_shift;
+    part.items = waves << part.split_shift;
+    part.blocks = std::min((part.items + kHeadsWaves - 1) / kHeadsWaves, most_blocks);
+}
 
 HeadsShape heads_shape(const ps_heads_call* c, bool backward)
 {
     HeadsShape s;
     HeadsArgs& a = s.a;
     memset(&a, 0, sizeof(a));
-    memcpy(a.x, c->x, sizeof(a.x));
-    memcpy(a.grad, c->grad, sizeof(a.grad));
-    memcpy(a.out, c->out, sizeof(a.out));
-    memcpy(a.weight, c->weight, sizeof(a.weight));
-    memcpy(a.x_stride, c->x_stride, sizeof(a.x_stride));
-    memcpy(a.grad_stride, c->grad_stride, sizeof(a.grad_stride));
     memcpy(a.position_stride, c->position_stride, sizeof(a.position_stride));
-    memcpy(a.heads, c->heads, sizeof(a.heads));
     a.positions = c->positions;
     a.plan = c->plan;
     a.tokens = (uint32_t)c->tokens;
@@ -110,20 +126,16 @@ HeadsShape heads_shape(const ps_heads_call* c, bool backward)
     a.weight_f32 = c->weight_dtype == PS_F32;
     a.positions_64 = c->position_bytes == 8;
     a.interleaved = c->interleaved != 0;
-    a.inverse = c->inverse != 0;
+    a.inverse = backward ? !c->inverse : c->inverse != 0;  // the gradient turns back
     s.v = 16 / size_of(c->dtype);
     while (!fits_vectors(c, s.v, backward)) s.v /= 2;
     const int units = (c->dim + 2 * s.v - 1) / (2 * s.v);
     while ((1 << a.group_shift) < units && a.group_shift < 6) ++a.group_shift;
-    const int heads = c->heads[0] + c->heads[1];
-    while ((1 << a.slot_shift) < heads && a.slot_shift < 6 - a.group_shift) ++a.slot_shift;
-    const int tokens_shift = 6 - a.group_shift - a.slot_shift;
-    s.waves = (a.all_tokens + (1u << tokens_shift) - 1) >> tokens_shift;
-    // few tokens: a token's heads are spread over more waves, each of which makes the token's angles for itself
-    const uint32_t turns = (uint32_t)((heads + (1 << a.slot_shift) - 1) >> a.slot_shift);
-    s.splits = 1;
-    while (s.splits < turns && s.waves * s.splits < 4 * kCus) s.splits *= 2;
-    s.splits = std::min({s.splits, turns, 65535u});
+    const uint32_t most = backward ? kBackwardBlocks : kForwardBlocks;
+    const int heads = std::max(1, c->heads[0] + c->heads[1]);
+    for (int which = 0; which < 2; ++which)
+        shape_part(c, which, a, std::max(1u, (uint32_t)((uint64_t)most * c->heads[which] / heads)), a.part[which]);
+    s.blocks = a.part[0].blocks + a.part[1].blocks;
     return s;
 }
 
@@ -141,12 +153,6 @@ void with_heads_kernel(int dtype, int v, F f)
     });
 }
 static_assert(PS_MAX_HEAD_DIM <= 2 * 4 * 64 && PS_MAX_HEAD_DIM <= 2 * 2 * 2 * 64 && PS_MAX_HEAD_DIM <= 2 * 64 * 4, "a group holds a head");
-
-uint32_t backward_blocks(const HeadsShape& s)
-{
-    const uint32_t blocks = (s.waves + kHeadsBlock / 64 - 1) / (kHeadsBlock / 64);
-    return std::min(blocks, std::max(1u, 4u * kCus / s.splits));
-}
 
 bool wants_weight_grad(const ps_heads_call* c)
 {
@@ -257,13 +263,13 @@ int ps_rotate_heads(const ps_heads_call* call, ps_stream_t stream)
     if (int rc = check_heads(call, false)) return rc;
     if (call->batch * call->tokens == 0 || call->heads[0] + call->heads[1] == 0) return 0;
     const HeadsShape s = heads_shape(call, false);
-    const dim3 grid((s.waves + kHeadsBlock / 64 - 1) / (kHeadsBlock / 64), s.splits);
     with_heads_kernel(call->dtype, s.v, [&](auto t, auto v, auto u) {
         typedef decltype(t) T;
+        const hipStream_t st = static_cast<hipStream_t>(stream);
         if (call->norm)
-            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), true>), grid, dim3(kHeadsBlock), 0, static_cast<hipStream_t>(stream), s.a);
+            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), true>), dim3(s.blocks), dim3(kHeadsBlock), 0, st, s.a);
         else
-            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), false>), grid, dim3(kHeadsBlock), 0, static_cast<hipStream_t>(stream), s.a);
+            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), false>), dim3(s.blocks), dim3(kHeadsBlock), 0, st, s.a);
     });
     PS_HIP(hipGetLastError());
     return 0;
@@ -272,8 +278,7 @@ int ps_rotate_heads(const ps_heads_call* call, ps_stream_t stream)
 size_t ps_norm_rotate_heads_workspace_bytes(const ps_heads_call* call)
 {
     if (check_heads(call, true) || call->batch * call->tokens == 0 || !wants_weight_grad(call)) return 0;
-    const HeadsShape s = heads_shape(call, true);
-    return (size_t)backward_blocks(s) * s.splits * 2 * (size_t)call->dim * sizeof(float);
+    return (size_t)heads_shape(call, true).blocks * (size_t)call->dim * sizeof(float);
 }
 
 int ps_norm_rotate_heads_backward(const ps_heads_call* call, void* d_workspace, size_t workspace_bytes, ps_stream_t stream)
@@ -283,26 +288,33 @@ int ps_norm_rotate_heads_backward(const ps_heads_call* call, void* d_workspace, 
     if (workspace_bytes < needed || (needed && (!d_workspace || (uintptr_t)d_workspace % 16)))
         return fail(PS_ERR_BAD_ARG, "the workspace has %zu bytes at %p, %zu are needed, 16-byte aligned", workspace_bytes, d_workspace, needed);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool empty = call->batch * call->tokens == 0;
-    uint32_t rows = 0;
-    if (!empty && call->heads[0] + call->heads[1] > 0) {
+    WeightGrads sums;
+    memset(&sums, 0, sizeof(sums));  // (of no tokens: zeros)
+    if (call->batch * call->tokens > 0 && call->heads[0] + call->heads[1] > 0) {
         HeadsShape s = heads_shape(call, true);
-        s.a.inverse = !call->inverse;  // the gradient turns back
-        s.a.partial = needed ? static_cast<float*>(d_workspace) : nullptr;
-        const dim3 grid(backward_blocks(s), s.splits);
-        rows = needed ? grid.x * grid.y : 0;
+        if (needed) {
+            float* partial = static_cast<float*>(d_workspace);
+            for (int which = 0; which < 2; ++which) {
+                sums.partial[which] = s.a.part[which].partial = partial;
+                sums.rows[which] = (int)s.a.part[which].blocks;
+                partial += (size_t)s.a.part[which].blocks * (size_t)call->dim;
+            }
+        }
         with_heads_kernel(call->dtype, s.v, [&](auto t, auto v, auto u) {
             typedef decltype(t) T;
-            hipLaunchKernelGGL((norm_rotate_heads_backward_kernel<T, v(), u()>), grid, dim3(kHeadsBlock), 0, st, s.a, s.waves);
+            hipLaunchKernelGGL((norm_rotate_heads_backward_kernel<T, v(), u()>), dim3(s.blocks), dim3(kHeadsBlock), 0, st, s.a);
         });
         PS_HIP(hipGetLastError());
     }
-    if (call->weight_grad[0] || call->weight_grad[1]) {  // (of no tokens: zeros)
+    if (call->weight_grad[0] || call->weight_grad[1]) {
+        sums.out[0] = call->weight_grad[0];
+        sums.out[1] = call->weight_grad[1];
+        sums.dim = call->dim;
+        sums.f32 = call->weight_dtype == PS_F32;
         with_type(call->dtype, [&](auto t) {
             typedef decltype(t) T;
-            hipLaunchKernelGGL((sum_weight_grads_kernel<T>), dim3((2 * call->dim + kSumColumns - 1) / kSumColumns), dim3(kSumColumns * kSumSlices),
-                               0, st, static_cast<const float*>(d_workspace), (int)rows, call->dim, call->weight_grad[0], call->weight_grad[1],
-                               call->weight_dtype == PS_F32);
+            hipLaunchKernelGGL((sum_weight_grads_kernel<T>), dim3((call->dim + kSumColumns - 1) / kSumColumns, 2), dim3(kSumColumns * kSumSlices),
+                               0, st, sums);
         });
         PS_HIP(hipGetLastError());
     }

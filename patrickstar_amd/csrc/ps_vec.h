@@ -46,30 +46,36 @@ struct VecOf<T, 1> {
 
 // V elements whose address is a multiple of their size.
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&out)[V])
+__device__ __forceinline__ typename VecOf<T, V>::type load_raw(const T* p)
 {
-    if constexpr (V == 1) {
-        out[0] = to_float<T>(*global(p));
-    } else {
-        typedef typename VecOf<T, V>::type vec;
-        const vec v = *global(reinterpret_cast<const vec*>(p));
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[e] = to_float<T>(v[e]);
-    }
+    return *global(reinterpret_cast<const typename VecOf<T, V>::type*>(p));
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_raw(T* p, typename VecOf<T, V>::type v)
+{
+    *global(reinterpret_cast<typename VecOf<T, V>::type*>(p)) = v;
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void store_vec(T* p, const float (&in)[V])
+__device__ __forceinline__ float element(typename VecOf<T, V>::type v, int e)
 {
-    if constexpr (V == 1) {
-        *global(p) = from_float<T>(in[0]);
-    } else {
-        typedef typename VecOf<T, V>::type vec;
-        vec v;
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = from_float<T>(in[e]);
-        *global(reinterpret_cast<vec*>(p)) = v;
-    }
+    if constexpr (V == 1)
+        return to_float<T>(v);
+    else
+        return to_float<T>(v[e]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void put(typename VecOf<T, V>::type& v, int e, T x)
+{
+    if constexpr (V == 1)
+        v = x;
+    else
+        v[e] = x;
+}
+template <typename T, int V>
+__device__ __forceinline__ void set_element(typename VecOf<T, V>::type& v, int e, float x)
+{
+    put<T, V>(v, e, from_float<T>(x));
 }
 
 }  // namespace
