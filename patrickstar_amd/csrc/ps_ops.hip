@@ -16,7 +16,8 @@ namespace {
 constexpr int kCus = 256;
 
 // Workgroups of the rotations, which loop over their tokens.
-constexpr uint32_t kForwardBlocks = 16 * kCus, kBackwardBlocks = 4 * kCus;
+constexpr uint32_t kForwardBlocks = 64 * kCus, kBackwardBlocks = 4 * kCus;
+constexpr int64_t kCachedBytes = 32 << 20;  // outputs up to so long are written through the L2 caches for whoever reads them next
 
 int size_of(int dtype) { return dtype == PS_F32 ? 4 : 2; }
 
@@ -86,6 +87,7 @@ struct HeadsShape {
     HeadsArgs a;
     int v;            // elements of a vector
     uint32_t blocks;  // of queries and keys together
+    bool stream;      // the outputs are longer than the caches
 };
 
 // A wave's items of queries or keys, and the workgroups that take them.
@@ -125,10 +127,13 @@ HeadsShape heads_shape(const ps_heads_call* c, bool backward)
     a.inv_dim = 1.0f / (float)c->dim;
     a.weight_f32 = c->weight_dtype == PS_F32;
     a.positions_64 = c->position_bytes == 8;
+    a.one_axis = c->axes == 1;
     a.interleaved = c->interleaved != 0;
     a.inverse = backward ? !c->inverse : c->inverse != 0;  // the gradient turns back
-    s.v = 16 / size_of(c->dtype);
+    // (8 bytes a lane of the 16-bit types: with 16, half as many waves fit a CU, and the norm's gradient took 131 us instead of 102)
+    s.v = 4;
     while (!fits_vectors(c, s.v, backward)) s.v /= 2;
+    a.whole = a.interleaved && fits_vectors(c, 2 * s.v, backward);
     const int units = (c->dim + 2 * s.v - 1) / (2 * s.v);
     while ((1 << a.group_shift) < units && a.group_shift < 6) ++a.group_shift;
     const uint32_t most = backward ? kBackwardBlocks : kForwardBlocks;
@@ -136,7 +141,18 @@ HeadsShape heads_shape(const ps_heads_call* c, bool backward)
     for (int which = 0; which < 2; ++which)
         shape_part(c, which, a, std::max(1u, (uint32_t)((uint64_t)most * c->heads[which] / heads)), a.part[which]);
     s.blocks = a.part[0].blocks + a.part[1].blocks;
+    s.stream = c->batch * c->tokens * (c->heads[0] + c->heads[1]) * (int64_t)c->dim * size_of(c->dtype) > kCachedBytes;
     return s;
+}
+
+// Calls f(first, second) with both as constants.
+template <typename F>
+void with_flags(bool first, bool second, F f)
+{
+    if (first && second) return f(std::true_type(), std::true_type());
+    if (first) return f(std::true_type(), std::false_type());
+    if (second) return f(std::false_type(), std::true_type());
+    f(std::false_type(), std::false_type());
 }
 
 // Calls f(type, vector length, units a lane).
@@ -144,15 +160,12 @@ template <typename F>
 void with_heads_kernel(int dtype, int v, F f)
 {
     with_type(dtype, [&](auto t) {
-        if constexpr (sizeof(t) == 2) {
-            if (v == 8) return f(t, Int<8>(), Int<1>());
-        }
         if (v == 4) return f(t, Int<4>(), Int<1>());
         if (v == 2) return f(t, Int<2>(), Int<2>());
         f(t, Int<1>(), Int<4>());
     });
 }
-static_assert(PS_MAX_HEAD_DIM <= 2 * 4 * 64 && PS_MAX_HEAD_DIM <= 2 * 2 * 2 * 64 && PS_MAX_HEAD_DIM <= 2 * 64 * 4, "a group holds a head");
+static_assert(PS_MAX_HEAD_DIM <= 2 * 4 * 64 && PS_MAX_HEAD_DIM <= 2 * 2 * 2 * 64 && PS_MAX_HEAD_DIM <= 2 * 1 * 4 * 64, "a group holds a head");
 
 bool wants_weight_grad(const ps_heads_call* c)
 {
@@ -266,10 +279,9 @@ int ps_rotate_heads(const ps_heads_call* call, ps_stream_t stream)
     with_heads_kernel(call->dtype, s.v, [&](auto t, auto v, auto u) {
         typedef decltype(t) T;
         const hipStream_t st = static_cast<hipStream_t>(stream);
-        if (call->norm)
-            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), true>), dim3(s.blocks), dim3(kHeadsBlock), 0, st, s.a);
-        else
-            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), false>), dim3(s.blocks), dim3(kHeadsBlock), 0, st, s.a);
+        with_flags(call->norm, s.stream, [&](auto norm, auto streamed) {
+            hipLaunchKernelGGL((rotate_heads_kernel<T, v(), u(), norm(), streamed()>), dim3(s.blocks), dim3(kHeadsBlock), 0, st, s.a);
+        });
     });
     PS_HIP(hipGetLastError());
     return 0;
@@ -302,7 +314,9 @@ int ps_norm_rotate_heads_backward(const ps_heads_call* call, void* d_workspace, 
         }
         with_heads_kernel(call->dtype, s.v, [&](auto t, auto v, auto u) {
             typedef decltype(t) T;
-            hipLaunchKernelGGL((norm_rotate_heads_backward_kernel<T, v(), u()>), dim3(s.blocks), dim3(kHeadsBlock), 0, st, s.a);
+            with_flags(s.stream, false, [&](auto streamed, auto) {
+                hipLaunchKernelGGL((norm_rotate_heads_backward_kernel<T, v(), u(), streamed()>), dim3(s.blocks), dim3(kHeadsBlock), 0, st, s.a);
+            });
         });
         PS_HIP(hipGetLastError());
     }

@@ -39,7 +39,9 @@ struct HeadsArgs {
     int dim, pairs;
     int group_shift;  // log2 of G
     float eps, inv_dim;
+    bool one_axis;    // the position need not wait for the plan
     bool weight_f32, positions_64, interleaved, inverse;
+    bool whole;       // every unit's two vectors are one, aligned as such
 };
 
 // cos and sin of `phase` / 2^32 turns.  The instructions take turns; over all of [-1/2, 1/2) in steps of 2^-24 their largest error is
@@ -105,15 +107,30 @@ template <typename T, int V>
 struct Raw {
     typename VecOf<T, V>::type a, b;
 
-    __device__ __forceinline__ void load(const T* row, const Unit& u)
+    // `whole`: the two are one vector of 2 V elements
+    __device__ __forceinline__ void load(const T* row, const Unit& u, bool whole)
     {
+        if (whole) {
+            const auto both = load_raw<T, 2 * V>(row + u.a);
+#pragma unroll
+            for (int e = 0; e < V; ++e) put<T, V>(a, e, both[e]), put<T, V>(b, e, both[V + e]);
+            return;
+        }
         a = load_raw<T, V>(row + u.a);
         b = u.b >= 0 ? load_raw<T, V>(row + u.b) : typename VecOf<T, V>::type{};
     }
-    __device__ __forceinline__ void store(T* row, const Unit& u) const
+    template <bool STREAM>
+    __device__ __forceinline__ void store(T* row, const Unit& u, bool whole) const
     {
-        store_raw<T, V>(row + u.a, a);
-        if (u.b >= 0) store_raw<T, V>(row + u.b, b);
+        if (whole) {
+            typename VecOf<T, 2 * V>::type both;
+#pragma unroll
+            for (int e = 0; e < V; ++e) both[e] = get<T, V>(a, e), both[V + e] = get<T, V>(b, e);
+            store_raw<T, 2 * V, STREAM>(row + u.a, both);
+            return;
+        }
+        store_raw<T, V, STREAM>(row + u.a, a);
+        if (u.b >= 0) store_raw<T, V, STREAM>(row + u.b, b);
     }
     __device__ __forceinline__ Halves<V> halves(const Unit& u) const
     {
@@ -150,7 +167,7 @@ __device__ __forceinline__ Halves<V> weight_of(const void* weight, bool vectors,
     const T* w = static_cast<const T*>(weight);
     Raw<T, V> r;
     if (vectors) {
-        r.load(w, u);
+        r.load(w, u, false);
     } else {
         r.b = typename VecOf<T, V>::type{};
 #pragma unroll
@@ -219,7 +236,7 @@ __device__ __forceinline__ void make_turns(const HeadsArgs& p, const HeadsPart& 
         const uint32_t slot = (uint32_t)i / (uint32_t)p.pairs, pair = (uint32_t)i % (uint32_t)p.pairs;
         const uint32_t token = item.first_token + slot;
         if (token >= p.all_tokens) break;
-        const int64_t step = global(p.plan)[2 * pair], axis = global(p.plan)[2 * pair + 1];
+        const int64_t step = global(p.plan)[2 * pair], axis = p.one_axis ? 0 : global(p.plan)[2 * pair + 1];
         const int64_t at = axis * p.position_stride[0] + (token / p.tokens) * p.position_stride[1] + (token % p.tokens) * p.position_stride[2];
         const int64_t position = p.positions_64 ? global(static_cast<const int64_t*>(p.positions))[at]
                                                 : global(static_cast<const int32_t*>(p.positions))[at];
@@ -253,7 +270,7 @@ __device__ __forceinline__ void turn(Halves<V>& x, const float (&c)[V], const fl
     }
 }
 
-template <typename T, int V, int U, bool NORM>
+template <typename T, int V, int U, bool NORM, bool STREAM>
 __global__ __launch_bounds__(kHeadsBlock) void rotate_heads_kernel(HeadsArgs p)
 {
     __shared__ float2 turns[kHeadsWaves][kTurns<V, U>];
@@ -279,7 +296,7 @@ __global__ __launch_bounds__(kHeadsBlock) void rotate_heads_kernel(HeadsArgs p)
         if (head < heads) {
 #pragma unroll
             for (int k = 0; k < U; ++k)
-                if (units[k].there) next[k].load(x + head * part.x_stride[2], units[k]);
+                if (units[k].there) next[k].load(x + head * part.x_stride[2], units[k], p.whole);
         }
         float c[U][V], s[U][V];
         make_turns<V, U>(p, part, item, units, turns[wave], c, s);
@@ -298,7 +315,7 @@ __global__ __launch_bounds__(kHeadsBlock) void rotate_heads_kernel(HeadsArgs p)
             if (head + item.step < heads) {
 #pragma unroll
                 for (int k = 0; k < U; ++k)
-                    if (units[k].there) next[k].load(x + (head + item.step) * part.x_stride[2], units[k]);
+                    if (units[k].there) next[k].load(x + (head + item.step) * part.x_stride[2], units[k], p.whole);
             }
             if (NORM) {
                 const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum(sum, p.group_shift), p.inv_dim, p.eps));
@@ -318,7 +335,7 @@ __global__ __launch_bounds__(kHeadsBlock) void rotate_heads_kernel(HeadsArgs p)
                 turn<V>(v[k], c[k], s[k]);
                 Raw<T, V> result;
                 result.set(v[k], units[k]);
-                result.store(out + (int64_t)head * p.dim, units[k]);
+                result.template store<STREAM>(out + (int64_t)head * p.dim, units[k], p.whole);
             }
         }
     }
@@ -328,7 +345,7 @@ __global__ __launch_bounds__(kHeadsBlock) void rotate_heads_kernel(HeadsArgs p)
 //   dw = sum over tokens and heads of dy x r,   dx = r (w dy - x r^2 mean(x w dy)).
 // The root is made again from x, which has to be read anyway.  A lane keeps its part of dw in registers over all heads and tokens
 // that it takes; a workgroup leaves one row of sums, and sum_weight_grads_kernel adds the rows in their order: no atomics.
-template <typename T, int V, int U>
+template <typename T, int V, int U, bool STREAM>
 __global__ __launch_bounds__(kHeadsBlock) void norm_rotate_heads_backward_kernel(HeadsArgs p)
 {
     __shared__ float2 turns[kHeadsWaves][kTurns<V, U>];
@@ -358,8 +375,8 @@ __global__ __launch_bounds__(kHeadsBlock) void norm_rotate_heads_backward_kernel
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 if (!units[k].there) continue;
-                next_x[k].load(x + head * part.x_stride[2], units[k]);
-                next_g[k].load(g + head * part.grad_stride[2], units[k]);
+                next_x[k].load(x + head * part.x_stride[2], units[k], p.whole);
+                next_g[k].load(g + head * part.grad_stride[2], units[k], p.whole);
             }
         }
         float c[U][V], s[U][V];
@@ -378,8 +395,8 @@ __global__ __launch_bounds__(kHeadsBlock) void norm_rotate_heads_backward_kernel
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
                     if (!units[k].there) continue;
-                    next_x[k].load(x + (head + item.step) * part.x_stride[2], units[k]);
-                    next_g[k].load(g + (head + item.step) * part.grad_stride[2], units[k]);
+                    next_x[k].load(x + (head + item.step) * part.x_stride[2], units[k], p.whole);
+                    next_g[k].load(g + (head + item.step) * part.grad_stride[2], units[k], p.whole);
                 }
             }
 #pragma unroll
@@ -409,7 +426,7 @@ __global__ __launch_bounds__(kHeadsBlock) void norm_rotate_heads_backward_kernel
                 }
                 Raw<T, V> result;
                 result.set(d[k], units[k]);
-                result.store(out + (int64_t)head * p.dim, units[k]);
+                result.template store<STREAM>(out + (int64_t)head * p.dim, units[k], p.whole);
             }
         }
     }
@@ -463,7 +480,15 @@ __global__ __launch_bounds__(kSumColumns * kSumSlices) void sum_weight_grads_ker
     if (p.out[which] == nullptr) return;
     float sum = 0.0f;
     if (at < p.dim)
-        for (int r = slice; r < p.rows[which]; r += kSumSlices) sum += global(p.partial[which])[(int64_t)r * p.dim + at];
+        for (int r = slice; r < p.rows[which]; r += 4 * kSumSlices) {
+            float part[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = r + k * kSumSlices;
+                part[k] = row < p.rows[which] ? global(p.partial[which])[(int64_t)row * p.dim + at] : 0.0f;
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+        }
     sums[slice][column] = sum;
     __syncthreads();
     if (slice != 0 || at >= p.dim) return;

@@ -50,10 +50,14 @@ __device__ __forceinline__ typename VecOf<T, V>::type load_raw(const T* p)
 {
     return *global(reinterpret_cast<const typename VecOf<T, V>::type*>(p));
 }
-template <typename T, int V>
+// STREAM: with the non-temporal hint
+template <typename T, int V, bool STREAM = false>
 __device__ __forceinline__ void store_raw(T* p, typename VecOf<T, V>::type v)
 {
-    *global(reinterpret_cast<typename VecOf<T, V>::type*>(p)) = v;
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(v, global(reinterpret_cast<typename VecOf<T, V>::type*>(p)));
+    else
+        *global(reinterpret_cast<typename VecOf<T, V>::type*>(p)) = v;
 }
 
 template <typename T, int V>
@@ -63,6 +67,14 @@ __device__ __forceinline__ float element(typename VecOf<T, V>::type v, int e)
         return to_float<T>(v);
     else
         return to_float<T>(v[e]);
+}
+template <typename T, int V>
+__device__ __forceinline__ T get(typename VecOf<T, V>::type v, int e)
+{
+    if constexpr (V == 1)
+        return v;
+    else
+        return v[e];
 }
 template <typename T, int V>
 __device__ __forceinline__ void put(typename VecOf<T, V>::type& v, int e, T x)
