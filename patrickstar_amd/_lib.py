@@ -285,6 +285,12 @@ def load():
         fn.restype = res
         fn.argtypes = args
     binding = _load_binding()
+    lib.ops = None  # the operators' compiled calls
+    if binding is not None and all(hasattr(binding, name) for name in _COMPILED_OPS):
+        entries = ("ps_rotate_heads", "ps_norm_rotate_heads_workspace_bytes", "ps_norm_rotate_heads_backward", "ps_top_logits", "ps_distill_loss",
+                   "ps_distill_loss_backward", "ps_last_error")
+        binding.ops_use(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in entries))
+        lib.ops = binding
     lib.compiled = None  # (a step looks here: a name that the library is asked for in vain costs 2 us)
     # adam_op.adam_update's arguments -> return code, or None where the call is not of the ordinary form (csrc/ps_binding.cpp)
     if binding is None:
@@ -295,6 +301,9 @@ def load():
             lib.compiled = _Compiled(binding, lib)
     _lib = lib
     return lib
+
+
+_COMPILED_OPS = ("ops_use", "ops_heads", "ops_top", "ops_distill")
 
 
 def _no_binding(*args):

@@ -9,7 +9,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 LIB_PATH = os.path.join(PKG_DIR, "libps_adam.so")
 SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("ps_adam.hip", "ps_ops.hip")]
-BINDING_SOURCE = os.path.join(PKG_DIR, "csrc", "ps_binding.cpp")
+BINDING_SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("ps_binding.cpp", "ps_ops_binding.cpp")]
 BINDING_PATH = os.path.join(PKG_DIR, "_binding.so")
 INCLUDE = os.path.join(ROOT, "include")
 
@@ -101,7 +101,7 @@ def _compile_binding(out, verbose):
         cmd += ["-I", path]
     for path in cpp_extension.include_paths():
         cmd += ["-isystem", path]
-    cmd += [BINDING_SOURCE, "-o", out]
+    cmd += [*BINDING_SOURCES, "-o", out]
     for path in cpp_extension.library_paths():
         cmd += ["-L", path]
     _run(cmd + ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"], verbose)

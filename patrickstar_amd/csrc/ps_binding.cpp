@@ -1,3 +1,5 @@
+// (The operators' calls are in ps_ops_binding.cpp.)
+//
 // What the host does again and again for a step, compiled: adam_update of the operator module and FP16Adam's whole-list steps from
 // Python arguments to the library without Python in between, and the look at every parameter's numbers.
 //
@@ -22,6 +24,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "ps_adam.h"
+#include "ps_ops_binding.h"
 
 namespace {
 
@@ -309,7 +312,9 @@ PyMethodDef methods[] = {
     {"adam_update", fast(adam_update), METH_FASTCALL, nullptr},   {"step_chunks", fast(step_chunks), METH_FASTCALL, nullptr},
     {"step_dynamic", fast(step_dynamic), METH_FASTCALL, nullptr}, {"quiet", quiet, METH_NOARGS, nullptr},
     {"same_flags", fast(same_flags), METH_FASTCALL, nullptr},     {"read_numbers", fast(read_numbers), METH_FASTCALL, nullptr},
-    {"write_steps", fast(write_steps), METH_FASTCALL, nullptr},   {nullptr, nullptr, 0, nullptr},
+    {"write_steps", fast(write_steps), METH_FASTCALL, nullptr},   {"ops_use", fast(ps_ops_use), METH_FASTCALL, nullptr},
+    {"ops_heads", fast(ps_ops_heads), METH_FASTCALL, nullptr},    {"ops_top", fast(ps_ops_top), METH_FASTCALL, nullptr},
+    {"ops_distill", fast(ps_ops_distill), METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, 0, methods, nullptr, nullptr, nullptr, nullptr};
 

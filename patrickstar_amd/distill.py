@@ -20,6 +20,7 @@ from . import _lib
 from .rotary import DTYPES
 
 REDUCTIONS = ("mean", "sum", "none")
+_REDUCTION_NUMBER = {name: i for i, name in enumerate(REDUCTIONS)}
 
 
 class TopLogits(NamedTuple):
@@ -36,6 +37,11 @@ def top_logits(logits, k, temperature=1.0):
     Equal logits are taken by their place, the lowest first; NaN counts as larger than every number.  fp16, bf16 or fp32 on
     the GPU, ``k`` up to 1024 (and the vocabulary).  Not differentiable: a teacher's logits are data.
     """
+    ops = _lib.load().ops
+    if ops is not None:
+        out = ops.ops_top(logits, k, temperature)
+        if out is not None:
+            return TopLogits(*out)
     rows = _logit_rows("top_logits", logits)
     vocab = logits.shape[-1]
     if isinstance(k, bool) or not isinstance(k, int) or not 1 <= k <= min(vocab, _lib.PS_MAX_TOP):
@@ -73,6 +79,12 @@ def distill_loss(logits, ids, teacher_logits, teacher_lse=None, labels=None, *, 
     ``grad_scale``: the factor that backward is going to arrive with (a number, or a tensor with one element on the GPU), if
     the caller knows it; the logits are then read once for loss and gradient.  Not with ``reduction="none"``.
     """
+    ops = _lib.load().ops
+    if ops is not None:
+        loss = ops.ops_distill(logits, ids, teacher_logits, teacher_lse, labels, label_weight, temperature, ignore_index,
+                               _REDUCTION_NUMBER.get(reduction), grad_scale)
+        if loss is not None:
+            return loss
     rows = _logit_rows("distill_loss", logits)
     options = _checked_options(logits, ids, teacher_logits, teacher_lse, labels, label_weight, temperature, ignore_index, reduction,
                                grad_scale)

@@ -52,16 +52,13 @@ class RotaryPlan:
         self.rotary_dim = rotary_dim
         self.interleaved = bool(interleaved)
         self.sections = sections
+        self.axes = len(sections)
         self.axis_of_pair = _dealt(sections) if cycled else [a for a, n in enumerate(sections) for _ in range(n)]
         self.steps = [_step(f) for f in inv_freq]
         if device is None:
             device = torch.device("cuda", torch.cuda.current_device())
         # one row a pair: step, axis
         self.table = torch.tensor([[s, a] for s, a in zip(self.steps, self.axis_of_pair)], dtype=torch.int64, device=device)
-
-    @property
-    def axes(self):
-        return len(self.sections)
 
     @property
     def device(self):
@@ -93,6 +90,9 @@ def rotate_qk(q, k, positions, plan):
     not contiguous is copied first.  ``k`` may be None.  ``positions``: int32 or int64, ``[batch, tokens]`` or what expands to
     it, with a dimension for the axes in front if the plan has several.
     """
+    out = _compiled(q, k, None, None, positions, plan, False, 0.0)
+    if out is not None:
+        return out
     q, k, positions = _checked("rotate_qk", q, k, positions, plan)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotate.apply(q, k, positions, plan)
@@ -106,6 +106,9 @@ def norm_rotate_qk(q, k, q_weight, k_weight, positions, plan, eps=1e-6):
     32 bits and the result is rounded once.  Gradients: of queries, keys and weights, the latter summed over tokens and heads
     in an order that does not change from call to call.
     """
+    out = _compiled(q, k, q_weight, k_weight, positions, plan, True, eps)
+    if out is not None:
+        return out
     q, k, positions = _checked("norm_rotate_qk", q, k, positions, plan)
     if not eps >= 0.0:
         raise ValueError(f"norm_rotate_qk: eps must not be negative, got {eps}")
@@ -113,6 +116,16 @@ def norm_rotate_qk(q, k, q_weight, k_weight, positions, plan, eps=1e-6):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _NormRotate.apply(q, k, q_weight, k_weight, positions, plan, float(eps))
     return _rotate(q, k, positions, plan, weights=(q_weight, k_weight), eps=float(eps))
+
+
+def _compiled(q, k, q_weight, k_weight, positions, plan, norm, eps):
+    """The call as csrc/ps_ops_binding.cpp makes it, or None where it is not of the ordinary form."""
+    if type(plan) is not RotaryPlan:
+        return None
+    ops = _lib.load().ops
+    if ops is None:
+        return None
+    return ops.ops_heads(q, k, q_weight, k_weight, positions, plan.table, plan.axes, plan.rotary_dim, plan.interleaved, norm, eps)
 
 
 # -------------------------------------------------------------------------------------------------------------- checks

@@ -11,8 +11,18 @@ import pytest
 import torch
 
 import patrickstar_amd as ps
+from patrickstar_amd import _lib
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["compiled", "general"], autouse=True)
+def way(request, monkeypatch):
+    """Both ways to the library: the binding's calls, and the Python ones that take over where a call is not of the ordinary form."""
+    lib = _lib.load()
+    assert lib.ops is not None
+    if request.param == "general":
+        monkeypatch.setattr(lib, "ops", None)
 
 HALF_ULP = {torch.half: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float: 2.0**-24}
 TINY = {torch.half: 2.0**-25, torch.bfloat16: 0.0, torch.float: 0.0}
@@ -288,6 +298,15 @@ def test_a_second_backward_and_a_changed_scale():
     (c,) = torch.autograd.grad(loss, z, scale)
     (want,) = torch.autograd.grad(ps.distill_loss(z, ids, values), z, scale)
     assert torch.equal(c, want)
+
+
+def test_a_gradient_is_not_differentiated_in_silence():
+    z = made((5, 900), torch.float, 1).requires_grad_()
+    ids, values, t = lists(z.detach(), 8, 2)
+    for ahead in (None, 1.0):
+        (g,) = torch.autograd.grad(ps.distill_loss(z, ids, values, grad_scale=ahead).square(), z, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate"):
+            g.square().sum().backward()
 
 
 def test_strides_and_dimensions_and_the_same_bits_again():

@@ -10,8 +10,18 @@ import pytest
 import torch
 
 import patrickstar_amd as ps
+from patrickstar_amd import _lib
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["compiled", "general"], autouse=True)
+def way(request, monkeypatch):
+    """Both ways to the library: the binding's calls, and the Python ones that take over where a call is not of the ordinary form."""
+    lib = _lib.load()
+    assert lib.ops is not None
+    if request.param == "general":
+        monkeypatch.setattr(lib, "ops", None)
 
 HALF_ULP = {torch.half: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float: 2.0**-24}
 TINY = {torch.half: 2.0**-25, torch.bfloat16: 0.0, torch.float: 0.0}  # half of the smallest number below the normal ones
@@ -269,6 +279,16 @@ def test_rows_of_zeros_infinities_and_nan_stay_their_own():
     out, _ = ps.norm_rotate_qk(x, None, None, None, positions[0, :1], plan)
     (g,) = torch.autograd.grad(out, x, torch.ones_like(x))
     assert g.isfinite().all()
+
+
+def test_a_gradient_is_not_differentiated_in_silence():
+    q, k, positions, plan = inputs((2, 6, 4, 2, 64, 64, False, None, False, False), torch.float)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    q = q.requires_grad_()
+    for out in (ps.rotate_qk(q, k, positions, plan)[0], ps.norm_rotate_qk(q, k, w, w, positions, plan)[0]):
+        (g,) = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate"):
+            g.sum().backward()
 
 
 def test_no_tokens_and_no_heads():
