@@ -254,6 +254,80 @@ __device__ __forceinline__ uint32_t order_of(float x)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// A thread's sum of exponentials under its own largest logit so far.
+template <typename T>
+struct OnlineSum {
+    typedef typename RowVec<T>::type vec;
+    static constexpr int VE = RowShape<T>::VE;
+    float top = -__builtin_inff(), sum = 0.0f;
+
+    __device__ __forceinline__ float part(float z, float c, float mc) const { return exp2_fast(__builtin_fmaf(z, c, -mc)); }
+    // `largest` of what comes next
+    __device__ __forceinline__ void raise(float largest, float factor)
+    {
+        if (!(largest > top)) return;
+        const float c = row_factor(largest, factor), mc = largest * c;
+        sum = top == -__builtin_inff() ? sum : sum * exp2_fast(__builtin_fmaf(top, c, -mc));
+        top = largest;
+    }
+    template <int BLOCK>
+    __device__ __forceinline__ void add_row(const RowData<T, 0, BLOCK>& data, const RowShape<T>& s, float factor)
+    {
+        constexpr int kAhead = 4;  // vectors on their way at a time
+        int v = threadIdx.x;
+        for (; v + (kAhead - 1) * BLOCK < s.vectors; v += kAhead * BLOCK) {
+            raw_t x[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) x[j] = s.vector_at(v + j * BLOCK);
+            add<kAhead>(x, factor);
+        }
+        for (; v < s.vectors; v += BLOCK) {
+            const raw_t x[1] = {s.vector_at(v)};
+            add<1>(x, factor);
+        }
+        if (data.lone_at >= 0) {
+            const float z = to_float<T>(data.lone);
+            raise(z, factor);
+            add_element(z, factor);
+        }
+    }
+    __device__ __forceinline__ void add_element(float z, float factor)
+    {
+        const float c = row_factor(top, factor);
+        if (top != -__builtin_inff())
+            sum += part(z, c, top * c);
+        else if (z != z)  // among nothing but -inf so far, which adds nothing
+            sum = z;
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const raw_t (&x)[N], float factor)
+    {
+        Largest<T> largest;
+#pragma unroll
+        for (int j = 0; j < N; ++j) largest.add(x[j]);
+        raise(largest.get(), factor);
+        const float c = row_factor(top, factor), mc = top * c;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const vec v = __builtin_bit_cast(vec, x[j]);
+            if (top == -__builtin_inff()) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) add_element(to_float<T>(v[e]), factor);
+                continue;
+            }
+            float all = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) all += part(to_float<T>(v[e]), c, mc);
+            sum += all;
+        }
+    }
+    // the sum under the row's largest logit instead, whose factor is c
+    __device__ __forceinline__ float under(float c, float mc) const
+    {
+        return top == -__builtin_inff() ? sum : sum * exp2_fast(__builtin_fmaf(top, c, -mc));
+    }
+};
+
 __device__ __forceinline__ float number_of(uint32_t order)
 {
     const uint32_t b = order & 0x80000000u ? order & 0x7FFFFFFFu : ~order;
@@ -262,14 +336,15 @@ __device__ __forceinline__ float number_of(uint32_t order)
     return x;  // (NaN: 0x7FFFFFFF)
 }
 
-constexpr int kTopCandidates = 4096;
-constexpr int kBounds = 16;  // that are tried at a time
+constexpr int kBounds = 16;      // that are tried at a time
+constexpr int kSlotBytes = 24576;  // of LDS for the vectors of threads that reach the bound
 
 // 1. Every thread's largest element.  The k-th largest of these bounds the k-th largest of the row from below (k threads have one
 //    at least as large), and few elements reach it: about k of them where k is small against the threads.  Any smaller bound does
 //    too, so the search for it (kBounds at a time, each counted by a wave over all threads' largest) ends where little more than k
 //    threads reach it.
-// 2. Only those threads' vectors hold candidates: they are read again, spread over all threads.
+// 2. Only those threads' vectors hold candidates: handed over in LDS (or read again, where they are more or were not kept), they are
+//    spread over all threads.
 // 3. A candidate's place is the number of larger ones.
 // Where too many reach the bound (long runs of equal logits), or NaN or infinities are in the row, the k-th largest (order, place)
 // is found bit by bit: all are different, so exactly k reach it.
@@ -281,7 +356,10 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
     constexpr int kWaves = BLOCK / 64, kPerWave = kBounds / kWaves;  // (BLOCK <= 1024)
     // low bits of an order that say nothing: the type's own mantissa is shorter than fp32's by so many
     constexpr int kLow = sizeof(T) == 4 ? 0 : __is_same(T, half_t) ? 13 : 16;
+    constexpr int kTopCandidates = BLOCK == 256 ? 1024 : 2048;
+    constexpr int kSlots = NV == 0 ? 0 : NV < 8 ? 192 : kSlotBytes / (16 * NV);
     __shared__ uint64_t found[kTopCandidates];
+    __shared__ raw_t slots[NV > 0 ? kSlots * NV : 1];  // of threads that reach the bound: their vectors
     __shared__ uint32_t largest[BLOCK];
     __shared__ uint16_t reaching[BLOCK];
     __shared__ int place_of[BLOCK];
@@ -296,7 +374,16 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
         const RowShape<T> shape(row, p.vocab);
         RowData<T, NV, BLOCK> data;
         data.load(shape);
-        const uint32_t mine = order_of(data.largest(shape));  // (of a thread without elements: -inf's)
+        // A row that is not kept is read once for both: a thread's sum goes by its own largest so far.
+        OnlineSum<T> online;
+        float my_top;
+        if constexpr (NV == 0) {
+            online.add_row(data, shape, p.factor);
+            my_top = online.top;
+        } else {
+            my_top = data.largest(shape);
+        }
+        const uint32_t mine = order_of(my_top);  // (of a thread without elements: -inf's)
         largest[threadIdx.x] = mine;
         if (threadIdx.x == 0) n_found = n_reaching = 0;
         {
@@ -313,16 +400,20 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
         const float m = number_of(most), c = row_factor(m, p.factor), mc = m * c;
         // the sum of exponentials; NaN where a logit is NaN or infinite
         float sum = 0.0f;
-        data.hide();
-        data.each(
-            shape,
-            [&](const vec& v, int) PS_INLINE {
-                float part = 0.0f;
+        if (NV == 0) {
+            sum = online.under(c, mc);
+        } else {
+            data.hide();
+            data.each(
+                shape,
+                [&](const vec& v, int) PS_INLINE {
+                    float part = 0.0f;
 #pragma unroll
-                for (int e = 0; e < VE; ++e) part += exp2_fast(__builtin_fmaf(to_float<T>(v[e]), c, -mc));
-                sum += part;
-            },
-            [&](T x, int) PS_INLINE { sum += exp2_fast(__builtin_fmaf(to_float<T>(x), c, -mc)); });
+                    for (int e = 0; e < VE; ++e) part += exp2_fast(__builtin_fmaf(to_float<T>(v[e]), c, -mc));
+                    sum += part;
+                },
+                [&](T x, int) PS_INLINE { sum += exp2_fast(__builtin_fmaf(to_float<T>(x), c, -mc)); });
+        }
         sum = wave_sum(sum);
         if (lane == 0) lds_sum[wave] = sum;
         // the bound: at least k threads reach `bound`, fewer than k `above`
@@ -331,34 +422,28 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
         if (p.k <= BLOCK) {
             const int enough = p.k + p.k / 4 + 8;
             int turn = 0;
+            uint32_t others[kWaves];
+#pragma unroll
+            for (int j = 0; j < kWaves; ++j) others[j] = largest[j * 64 + lane];
             while (reach > enough && above - bound > 1) {
                 const uint32_t step = (above - bound) / (kBounds + 1), left = (above - bound) % (kBounds + 1);
                 auto tried = [&](uint32_t i) PS_INLINE { return bound + step * (i + 1) + (left * (i + 1)) / (kBounds + 1); };
-                int n[kPerWave];
 #pragma unroll
-                for (int i = 0; i < kPerWave; ++i) n[i] = 0;
+                for (int i = 0; i < kPerWave; ++i) {
+                    const uint32_t limit = tried(wave * kPerWave + i);
+                    int n = 0;
 #pragma unroll
-                for (int j = 0; j < kWaves; ++j) {
-                    const uint32_t other = largest[j * 64 + lane];
-#pragma unroll
-                    for (int i = 0; i < kPerWave; ++i) n[i] += __popcll(__ballot(other >= tried(wave * kPerWave + i)));
-                }
-                if (lane == 0) {
-#pragma unroll
-                    for (int i = 0; i < kPerWave; ++i) lds_count[turn][wave * kPerWave + i] = n[i];
+                    for (int j = 0; j < kWaves; ++j) n += __popcll(__ballot(others[j] >= limit));
+                    if (lane == 0) lds_count[turn][wave * kPerWave + i] = n;
                 }
                 __syncthreads();
-                uint32_t new_bound = bound, new_above = above;
-#pragma unroll
-                for (int i = kBounds - 1; i >= 0; --i) {
-                    const int count = lds_count[turn][i];
-                    if (count >= p.k) {
-                        if (new_bound == bound && tried(i) > bound) new_bound = tried(i), reach = count;
-                    } else {
-                        new_above = tried(i);
-                    }
-                }
-                bound = new_bound, above = new_above;
+                // the bounds rise, so the ones that k threads reach are the first of them
+                const int count = lds_count[turn][lane & (kBounds - 1)];
+                const int reached = __popcll(__ballot(count >= p.k) & ((1u << kBounds) - 1));
+                const uint32_t new_bound = reached > 0 ? tried(reached - 1) : bound;
+                if (reached < kBounds) above = tried(reached);
+                if (reached > 0) reach = __builtin_amdgcn_readlane(count, reached - 1);
+                bound = new_bound;
                 turn ^= 1;
             }
         }
@@ -367,35 +452,69 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) sum += lds_sum[w];
         const bool ordinary = sum - sum == 0.0f;
+        auto entry_of = [](float x, int at) PS_INLINE { return (uint64_t)(order_of(x) >> kLow) << 32 | (0xFFFFFFFFu - (uint32_t)at); };
+        auto value_of = [](uint64_t entry) PS_INLINE {
+            const uint32_t order = (uint32_t)(entry >> 32) << kLow;
+            return number_of(order & 0x80000000u ? order : order | ((1u << kLow) - 1));
+        };
         auto keep = [&](uint64_t entry) PS_INLINE {
             const int at = atomicAdd(&n_found, 1);
             if (at < kTopCandidates) found[at] = entry;
         };
-        auto entry_of = [](float x, int at) PS_INLINE { return (uint64_t)(order_of(x) >> kLow) << 32 | (0xFFFFFFFFu - (uint32_t)at); };
+        // the elements of a vector that reach the limit: one addition for all of them
+        const float limit = number_of(bound);
+        auto keep_of = [&](const vec& x, int first) PS_INLINE {
+            uint32_t reaches = 0;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) reaches |= to_float<T>(x[e]) >= limit ? 1u << e : 0u;
+            if (!reaches) return;
+            int at = atomicAdd(&n_found, __popc(reaches));
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                if (!(reaches >> e & 1)) continue;
+                if (at < kTopCandidates) found[at] = entry_of(to_float<T>(x[e]), first + e);
+                ++at;
+            }
+        };
         bool few = ordinary && p.k <= BLOCK && reach <= 2 * p.k + 64;
         if (few) {
             const uint64_t reaches = __ballot(mine >= bound);
             int at = 0;
             if (lane == 0 && reaches) at = atomicAdd(&n_reaching, __popcll(reaches));
-            at = __shfl(at, 0);
-            if (mine >= bound) reaching[at + __popcll(reaches & ((1ull << lane) - 1))] = (uint16_t)threadIdx.x;
-            __syncthreads();
-            const float limit = number_of(bound);
-            const int each = (shape.vectors + BLOCK - 1) / BLOCK;  // vectors of a thread
-            const int items = n_reaching * (each + 1);
-            for (int i = threadIdx.x; i < items; i += BLOCK) {
-                const int owner = reaching[i / (each + 1)], part = i % (each + 1), v = part * BLOCK + owner;
-                if (part == each) {
-                    const int place = shape.lone_of(owner);
-                    if (place >= 0) {
-                        const float x = to_float<T>(*global(row + place));
-                        if (x >= limit) keep(entry_of(x, place));
-                    }
-                } else if (v < shape.vectors) {
-                    const vec x = __builtin_bit_cast(vec, shape.vector_at(v));
+            at = __builtin_amdgcn_readfirstlane(at) + __popcll(reaches & ((1ull << lane) - 1));
+            const bool handed = NV > 0 && reach <= kSlots;  // (all of the workgroup's threads agree)
+            if (mine >= bound) {
+                reaching[at] = (uint16_t)threadIdx.x;
+                if (handed) {
+                    const int thread = fresh_thread();
 #pragma unroll
-                    for (int e = 0; e < VE; ++e)
-                        if (to_float<T>(x[e]) >= limit) keep(entry_of(to_float<T>(x[e]), shape.element_of(v) + e));
+                    for (int i = 0; i < NV; ++i)
+                        if (i * BLOCK + thread < shape.vectors) slots[at * NV + i] = data.kept[i];
+                }
+                if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of(to_float<T>(data.lone), data.lone_at));
+            }
+            __syncthreads();
+            const int each = (shape.vectors + BLOCK - 1) / BLOCK;  // vectors of a thread
+            const int items = n_reaching * each;
+            if (handed) {
+                for (int i = threadIdx.x; i < items; i += BLOCK) {
+                    const int slot = i / each, part = i - slot * each, v = part * BLOCK + reaching[slot];
+                    if (v < shape.vectors) keep_of(__builtin_bit_cast(vec, slots[slot * NV + part]), shape.element_of(v));
+                }
+            } else {
+                constexpr int kAhead = 4;  // vectors on their way at a time
+                for (int first = threadIdx.x; first < items; first += kAhead * BLOCK) {
+                    raw_t x[kAhead];
+                    int v[kAhead];
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) {
+                        const int i = first + j * BLOCK, slot = i / each;
+                        v[j] = i < items ? (i - slot * each) * BLOCK + reaching[slot] : shape.vectors;
+                        if (v[j] < shape.vectors) x[j] = shape.vector_at(v[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j)
+                        if (v[j] < shape.vectors) keep_of(__builtin_bit_cast(vec, x[j]), shape.element_of(v[j]));
                 }
             }
             __syncthreads();
@@ -450,12 +569,18 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
             if (!ordinary) {  // the row's largest, NaN being larger than everything: a row of -inf alone has no mass
                 uint64_t first = 0;
                 for (int i = 0; i < n; ++i) first = found[i] > first ? found[i] : first;
-                const uint32_t order = (uint32_t)(first >> 32) << kLow;
-                lse = number_of(order & 0x80000000u ? order : order | ((1u << kLow) - 1));
-                if (order == 0xFFFFFFFFu >> kLow << kLow) lse = __builtin_nanf("");
+                lse = (uint32_t)(first >> 32) == 0xFFFFFFFFu >> kLow ? __builtin_nanf("") : value_of(first);
             }
             *global(p.lse + r) = lse;
         }
+        auto write = [&](uint64_t entry, int place) PS_INLINE {
+            const uint32_t at = 0xFFFFFFFFu - (uint32_t)entry;
+            const float x = value_of(entry);
+            T value = from_float<T>(x);
+            if (!(x < 0.0f || x > 0.0f)) value = *global(row + at);  // a zero's sign, a NaN's bits
+            *global(p.ids + r * p.k + place) = (int32_t)at;
+            *global(static_cast<T*>(p.values) + r * p.k + place) = value;
+        };
         if (n <= BLOCK) {
             int span = 64;
             while (span < n) span *= 2;
@@ -463,28 +588,20 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
             place_of[threadIdx.x] = 0;
             __syncthreads();
             const uint64_t entry = mine_at < n ? found[mine_at] : 0;
-            if (mine_at < n) {
-                int count = 0;
-                for (int j = slice; j < n; j += slices) count += found[j] > entry;
-                if (count) atomicAdd(&place_of[mine_at], count);
-            }
+            int count = 0;
+#pragma unroll 4
+            for (int j = slice; j < n; j += slices) count += found[j] > entry;
+            if (mine_at < n && count) atomicAdd(&place_of[mine_at], count);
             __syncthreads();
             const int place = place_of[mine_at];
-            if (slice == 0 && mine_at < n && place < p.k) {
-                const uint32_t at = 0xFFFFFFFFu - (uint32_t)entry;
-                *global(p.ids + r * p.k + place) = (int32_t)at;
-                *global(static_cast<T*>(p.values) + r * p.k + place) = *global(row + at);
-            }
+            if (slice == 0 && mine_at < n && place < p.k) write(entry, place);
         } else {
             for (int i = threadIdx.x; i < n; i += BLOCK) {
                 const uint64_t entry = found[i];
                 int place = 0;
+#pragma unroll 4
                 for (int j = 0; j < n; ++j) place += found[j] > entry;
-                if (place < p.k) {
-                    const uint32_t at = 0xFFFFFFFFu - (uint32_t)entry;
-                    *global(p.ids + r * p.k + place) = (int32_t)at;
-                    *global(static_cast<T*>(p.values) + r * p.k + place) = *global(row + at);
-                }
+                if (place < p.k) write(entry, place);
             }
         }
     }
