@@ -180,32 +180,29 @@ struct RowData {
 
 // ------------------------------------------------------------------------------------------------------------ reductions
 
-__device__ __forceinline__ float wave_sum(float v)
+// Of all lanes of a wave, the same in every one: within 16 lanes by moves between lanes as part of the operation, then of the four
+// sixteens.
+template <typename N, typename F>
+__device__ __forceinline__ N wave_fold(N v, F f)
 {
-#pragma unroll
-    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-    return v;
+    v = f(v, moved<0xB1>(v));   // the other of a pair
+    v = f(v, moved<0x4E>(v));   // the other pair of four
+    v = f(v, moved<0x141>(v));  // mirrored in eight: fours are alike by now
+    v = f(v, moved<0x140>(v));  // mirrored in sixteen
+    return f(f(of_lane(v, 0), of_lane(v, 16)), f(of_lane(v, 32), of_lane(v, 48)));
+}
+template <typename N>
+__device__ __forceinline__ N wave_sum(N v)
+{
+    return wave_fold(v, [](N a, N b) { return a + b; });
 }
 __device__ __forceinline__ float wave_max(float v)
 {
-#pragma unroll
-    for (int m = 32; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
-    return v;
+    return wave_fold(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ uint32_t wave_max(uint32_t v)
 {
-#pragma unroll
-    for (int m = 32; m; m >>= 1) {
-        const uint32_t o = __shfl_xor(v, m);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-__device__ __forceinline__ int wave_sum(int v)
-{
-#pragma unroll
-    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-    return v;
+    return wave_fold(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
 // Every thread gets the result.  Each use needs LDS of its own, or a barrier between the uses.
@@ -337,37 +334,89 @@ __device__ __forceinline__ float number_of(uint32_t order)
 }
 
 constexpr int kBounds = 16;      // that are tried at a time
-constexpr int kSlotBytes = 24576;  // of LDS for the vectors of threads that reach the bound
+
+// Low bits of an order that say nothing: the type's own mantissa is shorter than fp32's by so many.
+template <typename T>
+constexpr int kLowBits = sizeof(T) == 4 ? 0 : __is_same(T, half_t) ? 13 : 16;
+
+// What candidates are told apart and ordered by: order, then place, the lower first.
+template <typename T>
+__device__ __forceinline__ uint64_t entry_of(float x, int at)
+{
+    return (uint64_t)(order_of(x) >> kLowBits<T>) << 32 | (0xFFFFFFFFu - (uint32_t)at);
+}
+
+// The k largest entries of a row, whatever it holds, found bit by bit.  The row is read again for every bit: what it takes is no
+// ordinary row's concern, and it needs no registers.  (n_found: 0 by now.)
+template <typename T, int BLOCK>
+__device__ __forceinline__ void keep_exactly(const T* row, int vocab, int k, uint64_t* found, int* n_found, int* counts)
+{
+    typedef typename RowVec<T>::type vec;
+    constexpr int VE = RowShape<T>::VE;
+    const RowShape<T> shape(row, vocab);
+    RowData<T, 0, BLOCK> data;
+    data.load(shape);
+    __syncthreads();
+    const int place_bits = 32 - __builtin_clz((uint32_t)vocab);
+    uint64_t kth = 0;
+    int turn = 0;
+    for (int bit = 63 - kLowBits<T>; bit >= 0; --bit) {
+        const uint64_t next = kth | 1ull << bit;
+        if (bit < 32 && bit >= place_bits) {  // every entry has these
+            kth = next;
+            continue;
+        }
+        int count = 0;
+        data.each(
+            shape,
+            [&](const vec& v, int i) PS_INLINE {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) count += entry_of<T>(to_float<T>(v[e]), shape.element_of(i) + e) >= next;
+            },
+            [&](T x, int at) PS_INLINE { count += entry_of<T>(to_float<T>(x), at) >= next; });
+        count = block_sum<BLOCK>(count, counts + turn * kBounds);
+        turn ^= 1;
+        if (count >= k) kth = next;
+        if (count == k) break;
+    }
+    auto keep = [&](uint64_t entry) PS_INLINE {
+        if (entry >= kth) found[atomicAdd(n_found, 1)] = entry;  // (k of them)
+    };
+    data.each(
+        shape,
+        [&](const vec& v, int i) PS_INLINE {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) keep(entry_of<T>(to_float<T>(v[e]), shape.element_of(i) + e));
+        },
+        [&](T x, int at) PS_INLINE { keep(entry_of<T>(to_float<T>(x), at)); });
+}
 
 // 1. Every thread's largest element.  The k-th largest of these bounds the k-th largest of the row from below (k threads have one
 //    at least as large), and few elements reach it: about k of them where k is small against the threads.  Any smaller bound does
 //    too, so the search for it (kBounds at a time, each counted by a wave over all threads' largest) ends where little more than k
 //    threads reach it.
-// 2. Only those threads' vectors hold candidates: handed over in LDS (or read again, where they are more or were not kept), they are
-//    spread over all threads.
+// 2. Only those threads' vectors can hold candidates: the ones that do are handed over in LDS and spread over all threads.
 // 3. A candidate's place is the number of larger ones.
-// Where too many reach the bound (long runs of equal logits), or NaN or infinities are in the row, the k-th largest (order, place)
-// is found bit by bit: all are different, so exactly k reach it.
+// Where too many reach the bound (long runs of equal logits), or NaN or infinities are in the row, keep_exactly finds the k-th largest
+// (order, place) bit by bit: all are different, so exactly k reach it.
 template <typename T, int NV, int BLOCK>
-__global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
+__global__ __launch_bounds__(BLOCK, BLOCK == 512 && NV <= 14 ? 6 : 4) void top_logits_kernel(TopArgs p)
 {
     typedef typename RowVec<T>::type vec;
     constexpr int VE = RowShape<T>::VE;
     constexpr int kWaves = BLOCK / 64, kPerWave = kBounds / kWaves;  // (BLOCK <= 1024)
-    // low bits of an order that say nothing: the type's own mantissa is shorter than fp32's by so many
-    constexpr int kLow = sizeof(T) == 4 ? 0 : __is_same(T, half_t) ? 13 : 16;
-    constexpr int kTopCandidates = BLOCK == 256 ? 1024 : 2048;
-    constexpr int kSlots = NV == 0 ? 0 : NV < 8 ? 192 : kSlotBytes / (16 * NV);
+    constexpr int kTopCandidates = BLOCK == 256 ? 512 : 2048;
+    constexpr int kSlots = NV == 0 ? BLOCK : BLOCK == 256 ? 256 : 1024;
     __shared__ uint64_t found[kTopCandidates];
-    __shared__ raw_t slots[NV > 0 ? kSlots * NV : 1];  // of threads that reach the bound: their vectors
+    __shared__ raw_t slots[NV > 0 ? kSlots : 1];  // vectors that hold candidates
+    __shared__ int slot_vector[kSlots];           // their numbers (of a row that is not kept: threads that have candidates)
     __shared__ uint32_t largest[BLOCK];
-    __shared__ uint16_t reaching[BLOCK];
     __shared__ int place_of[BLOCK];
     __shared__ uint32_t lds_max[kWaves], lds_min[kWaves];
     __shared__ float lds_sum[kWaves];
-    __shared__ int lds_count[2][kBounds];
-    __shared__ int n_found, n_reaching;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ int lds_count[2][kBounds];  // (as many as waves, at least)
+    __shared__ int n_found, n_slots;
+    const int thread = threadIdx.x, lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     {
         const int64_t r = p.first_row + blockIdx.x;
         const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
@@ -384,8 +433,8 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
             my_top = data.largest(shape);
         }
         const uint32_t mine = order_of(my_top);  // (of a thread without elements: -inf's)
-        largest[threadIdx.x] = mine;
-        if (threadIdx.x == 0) n_found = n_reaching = 0;
+        largest[thread] = mine;
+        if (thread == 0) n_found = n_slots = 0;
         {
             const uint32_t hi = wave_max(mine), lo = ~wave_max(~mine);
             if (lane == 0) lds_max[wave] = hi, lds_min[wave] = lo;
@@ -452,10 +501,9 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) sum += lds_sum[w];
         const bool ordinary = sum - sum == 0.0f;
-        auto entry_of = [](float x, int at) PS_INLINE { return (uint64_t)(order_of(x) >> kLow) << 32 | (0xFFFFFFFFu - (uint32_t)at); };
         auto value_of = [](uint64_t entry) PS_INLINE {
-            const uint32_t order = (uint32_t)(entry >> 32) << kLow;
-            return number_of(order & 0x80000000u ? order : order | ((1u << kLow) - 1));
+            const uint32_t order = (uint32_t)(entry >> 32) << kLowBits<T>;
+            return number_of(order & 0x80000000u ? order : order | ((1u << kLowBits<T>) - 1));
         };
         auto keep = [&](uint64_t entry) PS_INLINE {
             const int at = atomicAdd(&n_found, 1);
@@ -472,104 +520,93 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
                 if (!(reaches >> e & 1)) continue;
-                if (at < kTopCandidates) found[at] = entry_of(to_float<T>(x[e]), first + e);
+                if (at < kTopCandidates) found[at] = entry_of<T>(to_float<T>(x[e]), first + e);
                 ++at;
             }
         };
         bool few = ordinary && p.k <= BLOCK && reach <= 2 * p.k + 64;
-        if (few) {
+        if (few && NV > 0) {
+            // a thread that reaches the bound leaves those of its vectors that do
+            if (mine >= bound) {
+                uint32_t reaches = 0;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    Largest<T> top;
+                    top.add(data.kept[i]);
+                    if (i * BLOCK + thread < shape.vectors && top.get() >= limit) reaches |= 1u << i;
+                }
+                if (reaches) {
+                    int at = atomicAdd(&n_slots, __popc(reaches));
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        if (!(reaches >> i & 1)) continue;
+                        if (at < kSlots) slots[at] = data.kept[i], slot_vector[at] = i * BLOCK + thread;
+                        ++at;
+                    }
+                }
+                if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of<T>(to_float<T>(data.lone), data.lone_at));
+            }
+            __syncthreads();
+            const int n = n_slots;
+            few = n <= kSlots;
+            // an element a thread, and one addition a wave
+            const T* elements = reinterpret_cast<const T*>(slots);
+            for (int first = wave * 64; few && first < n * VE; first += BLOCK) {
+                const int i = first + lane;
+                const float x = i < n * VE ? to_float<T>(elements[i]) : 0.0f;
+                const bool reaches = i < n * VE && x >= limit;
+                const uint64_t all = __ballot(reaches);
+                int at = 0;
+                if (lane == 0 && all) at = atomicAdd(&n_found, __popcll(all));
+                at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
+                if (reaches && at < kTopCandidates) found[at] = entry_of<T>(x, shape.element_of(slot_vector[i / VE]) + i % VE);
+            }
+            __syncthreads();
+            few = few && n_found <= kTopCandidates;
+        } else if (few) {
+            // of a row that is not kept, the vectors of threads that reach the bound are read again, spread over all threads
             const uint64_t reaches = __ballot(mine >= bound);
             int at = 0;
-            if (lane == 0 && reaches) at = atomicAdd(&n_reaching, __popcll(reaches));
+            if (lane == 0 && reaches) at = atomicAdd(&n_slots, __popcll(reaches));
             at = __builtin_amdgcn_readfirstlane(at) + __popcll(reaches & ((1ull << lane) - 1));
-            const bool handed = NV > 0 && reach <= kSlots;  // (all of the workgroup's threads agree)
             if (mine >= bound) {
-                reaching[at] = (uint16_t)threadIdx.x;
-                if (handed) {
-                    const int thread = fresh_thread();
-#pragma unroll
-                    for (int i = 0; i < NV; ++i)
-                        if (i * BLOCK + thread < shape.vectors) slots[at * NV + i] = data.kept[i];
-                }
-                if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of(to_float<T>(data.lone), data.lone_at));
+                slot_vector[at] = thread;
+                if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of<T>(to_float<T>(data.lone), data.lone_at));
             }
             __syncthreads();
             const int each = (shape.vectors + BLOCK - 1) / BLOCK;  // vectors of a thread
-            const int items = n_reaching * each;
-            if (handed) {
-                for (int i = threadIdx.x; i < items; i += BLOCK) {
-                    const int slot = i / each, part = i - slot * each, v = part * BLOCK + reaching[slot];
-                    if (v < shape.vectors) keep_of(__builtin_bit_cast(vec, slots[slot * NV + part]), shape.element_of(v));
-                }
-            } else {
-                constexpr int kAhead = 4;  // vectors on their way at a time
-                for (int first = threadIdx.x; first < items; first += kAhead * BLOCK) {
-                    raw_t x[kAhead];
-                    int v[kAhead];
+            const int items = n_slots * each;
+            constexpr int kAhead = 4;  // vectors on their way at a time
+            for (int first = thread; first < items; first += kAhead * BLOCK) {
+                raw_t x[kAhead];
+                int v[kAhead];
 #pragma unroll
-                    for (int j = 0; j < kAhead; ++j) {
-                        const int i = first + j * BLOCK, slot = i / each;
-                        v[j] = i < items ? (i - slot * each) * BLOCK + reaching[slot] : shape.vectors;
-                        if (v[j] < shape.vectors) x[j] = shape.vector_at(v[j]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j)
-                        if (v[j] < shape.vectors) keep_of(__builtin_bit_cast(vec, x[j]), shape.element_of(v[j]));
+                for (int j = 0; j < kAhead; ++j) {
+                    const int i = first + j * BLOCK, slot = i / each;
+                    v[j] = i < items ? (i - slot * each) * BLOCK + slot_vector[slot] : shape.vectors;
+                    asm volatile("" : "=v"(x[j]));
+                    if (v[j] < shape.vectors) x[j] = shape.vector_at(v[j]);
                 }
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    if (v[j] < shape.vectors) keep_of(__builtin_bit_cast(vec, x[j]), shape.element_of(v[j]));
             }
             __syncthreads();
             few = n_found <= kTopCandidates;
         }
         if (!few) {
-            // the row is read again for every bit: what it takes is no ordinary row's concern, and it needs no registers
-            RowData<T, 0, BLOCK> again;
-            again.load(shape);
-            __syncthreads();
-            const int place_bits = 32 - __builtin_clz((uint32_t)p.vocab);
-            uint64_t kth = 0;
-            int turn = 0;
-            for (int bit = 63 - kLow; bit >= 0; --bit) {
-                const uint64_t next = kth | 1ull << bit;
-                if (bit < 32 && bit >= place_bits) {  // every entry has these
-                    kth = next;
-                    continue;
-                }
-                int count = 0;
-                again.each(
-                    shape,
-                    [&](const vec& v, int i) PS_INLINE {
-#pragma unroll
-                        for (int e = 0; e < VE; ++e) count += entry_of(to_float<T>(v[e]), shape.element_of(i) + e) >= next;
-                    },
-                    [&](T x, int at) PS_INLINE { count += entry_of(to_float<T>(x), at) >= next; });
-                count = block_sum<BLOCK>(count, lds_count[turn]);
-                turn ^= 1;
-                if (count >= p.k) kth = next;
-                if (count == p.k) break;
-            }
-            if (threadIdx.x == 0) n_found = 0;
-            __syncthreads();
-            again.each(
-                shape,
-                [&](const vec& v, int i) PS_INLINE {
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        const uint64_t entry = entry_of(to_float<T>(v[e]), shape.element_of(i) + e);
-                        if (entry >= kth) keep(entry);
-                    }
-                },
-                [&](T x, int at) PS_INLINE {
-                    if (entry_of(to_float<T>(x), at) >= kth) keep(entry_of(to_float<T>(x), at));
-                });
+            __syncthreads();  // everyone has seen how many there were
+            if (thread == 0) n_found = 0;
+            keep_exactly<T, BLOCK>(row, p.vocab, p.k, found, &n_found, lds_count[0]);
             __syncthreads();
         }
         const int n = n_found;
-        if (threadIdx.x == 0) {
+        if (thread == 0) {
             float lse = c == p.factor ? (mc + __builtin_amdgcn_logf(sum)) * kLn2 : m / p.temperature;
             if (!ordinary) {  // the row's largest, NaN being larger than everything: a row of -inf alone has no mass
                 uint64_t first = 0;
                 for (int i = 0; i < n; ++i) first = found[i] > first ? found[i] : first;
-                lse = (uint32_t)(first >> 32) == 0xFFFFFFFFu >> kLow ? __builtin_nanf("") : value_of(first);
+                lse = (uint32_t)(first >> 32) == 0xFFFFFFFFu >> kLowBits<T> ? __builtin_nanf("") : value_of(first);
             }
             *global(p.lse + r) = lse;
         }
@@ -584,8 +621,8 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
         if (n <= BLOCK) {
             int span = 64;
             while (span < n) span *= 2;
-            const int slices = BLOCK / span, mine_at = threadIdx.x & (span - 1), slice = threadIdx.x / span;
-            place_of[threadIdx.x] = 0;
+            const int slices = BLOCK / span, mine_at = thread & (span - 1), slice = thread / span;
+            place_of[thread] = 0;
             __syncthreads();
             const uint64_t entry = mine_at < n ? found[mine_at] : 0;
             int count = 0;
@@ -596,7 +633,7 @@ __global__ __launch_bounds__(BLOCK, 4) void top_logits_kernel(TopArgs p)
             const int place = place_of[mine_at];
             if (slice == 0 && mine_at < n && place < p.k) write(entry, place);
         } else {
-            for (int i = threadIdx.x; i < n; i += BLOCK) {
+            for (int i = thread; i < n; i += BLOCK) {
                 const uint64_t entry = found[i];
                 int place = 0;
 #pragma unroll 4

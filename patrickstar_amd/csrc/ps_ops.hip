@@ -188,6 +188,9 @@ void with_row(int vocab, int threads, F f)
     }
     if (threads <= 512) {
         if (vectors <= 4096) return f(Int<8>(), Int<512>());
+        // (a few registers less are a workgroup more on a CU)
+        if (vectors <= 6144) return f(Int<12>(), Int<512>());
+        if (vectors <= 7168) return f(Int<14>(), Int<512>());
         if (vectors <= 8192) return f(Int<16>(), Int<512>());
     }
     if (vectors <= 4096) return f(Int<4>(), Int<1024>());

@@ -55,11 +55,6 @@ __device__ __forceinline__ void cos_sin(int32_t phase, float& c, float& s)
 
 // Sum over the lanes of a group; every lane gets it.  Within 16 lanes by moves between lanes as part of the addition, which take
 // no LDS.
-template <int CTRL>
-__device__ __forceinline__ float moved(float v)
-{
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
-}
 __device__ __forceinline__ float group_sum(float v, int group_shift)
 {
     if (group_shift > 0) v += moved<0xB1>(v);   // the other of a pair

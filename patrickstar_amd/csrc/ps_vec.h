@@ -90,6 +90,18 @@ __device__ __forceinline__ void set_element(typename VecOf<T, V>::type& v, int e
     put<T, V>(v, e, from_float<T>(x));
 }
 
+// A value (32 bits) of another lane of the same 16, as CTRL says, and of one lane for the whole wave.  (All lanes take part.)
+template <int CTRL, typename N>
+__device__ __forceinline__ N moved(N v)
+{
+    return __builtin_bit_cast(N, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+template <typename N>
+__device__ __forceinline__ N of_lane(N v, int lane)
+{
+    return __builtin_bit_cast(N, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
 }  // namespace
 
 #endif  // PS_VEC_H
