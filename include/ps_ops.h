@@ -102,7 +102,7 @@ typedef struct ps_distill_call {
     float* row_loss;             /* rows */
     float* stats;                /* rows x 4: what the backward pass needs (NULL: not wanted) */
     float* loss;                 /* 1: the rows' sum, over `denominator`; NULL: not wanted */
-    float* denominator;          /* 1: number of rows that count (at least 1), made here for `mean`; NULL: 1 */
+    float* denominator;          /* 1, with `mean`: the number of rows that count (at least 1) is left here for the backward pass */
     void* grad;                  /* gradient of the logits, contiguous; NULL: not wanted */
     const float* upstream;       /* what the gradient is multiplied by; NULL: upstream_value */
     float* upstream_used;        /* 1: the factor that `grad` was made with (NULL: not wanted) */

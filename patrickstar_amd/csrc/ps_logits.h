@@ -654,7 +654,7 @@ struct DistillArgs {
     const void* labels;
     float* row_loss;
     float* stats;
-    const float* denominator;
+    float* denominator;   // rows that count: made here (count_rows), or before; nullptr: `count`
     void* grad;
     const float* upstream;
     float* upstream_used;
@@ -662,8 +662,9 @@ struct DistillArgs {
     int64_t ignore_index;
     int vocab, k;
     int values_dtype;
-    float temperature, label_weight, upstream_value;
+    float temperature, label_weight, upstream_value, count;
     bool ids_64, labels_64;
+    bool count_rows;      // few enough for every workgroup to count them itself
 };
 
 __device__ __forceinline__ int64_t whole_at(const void* p, int64_t at, bool is64)
@@ -897,7 +898,15 @@ __global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
     const bool soft = p.label_weight != 1.0f, hard = p.label_weight != 0.0f;
     const float upstream = p.upstream ? *global(p.upstream) : p.upstream_value;
     if (p.upstream_used && p.first_row + blockIdx.x == 0 && threadIdx.x == 0) *global(p.upstream_used) = upstream;
-    const float inv_count = p.denominator ? 1.0f / *global(p.denominator) : 1.0f;
+    float count = p.denominator && !p.count_rows ? *global(p.denominator) : p.count;
+    if (p.count_rows) {
+        int n = 0;
+        for (int i = threadIdx.x; i < (int)p.rows; i += BLOCK) n += whole_at(p.labels, i, p.labels_64) != p.ignore_index;
+        n = block_sum<BLOCK>(n, reinterpret_cast<int*>(lds[5]));
+        count = (float)(n > 0 ? n : 1);
+        if (p.first_row + blockIdx.x == 0 && threadIdx.x == 0) *global(p.denominator) = count;
+    }
+    const float inv_count = 1.0f / count;
     {
         const int64_t r = p.first_row + blockIdx.x;
         const RowShape<T> shape(static_cast<const T*>(p.logits) + r * p.row_stride, p.vocab);
@@ -1017,14 +1026,13 @@ __global__ __launch_bounds__(BLOCK) void distill_backward_kernel(DistillArgs p)
     if (p.upstream_used && *global(p.upstream) == *global(p.upstream_used)) return;
     int* ids = reinterpret_cast<int*>(dynamic);
     float* prob = reinterpret_cast<float*>(dynamic + p.k);
-    const float inv_count = p.denominator ? 1.0f / *global(p.denominator) : 1.0f;
-    {
-        const int64_t r = p.first_row + blockIdx.x;
+    const float inv_count = 1.0f / (p.denominator ? *global(p.denominator) : p.count);
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const RowShape<T> shape(static_cast<const T*>(p.logits) + r * p.row_stride, p.vocab);
         const int64_t label = p.labels ? whole_at(p.labels, r, p.labels_64) : -1;
         if (p.labels && label == p.ignore_index) {
             write_zeros<T, 0, BLOCK>(p, r, shape);
-            return;
+            continue;
         }
         RowStats s;
         s.m = *global(p.stats + 4 * r);
@@ -1036,6 +1044,7 @@ __global__ __launch_bounds__(BLOCK) void distill_backward_kernel(DistillArgs p)
         RowData<T, 0, BLOCK> data;
         data.load(shape);
         write_gradient<T, 0, BLOCK>(p, r, shape, data, s, *global(p.upstream + r * p.upstream_stride) * inv_count, ids, prob, label);
+        __syncthreads();  // before the next row's list
     }
 }
 
@@ -1044,13 +1053,13 @@ __global__ __launch_bounds__(1024) void count_rows_kernel(const void* labels, bo
 {
     __shared__ int lds[16];
     int n = 0;
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) n += labels == nullptr || whole_at(labels, r, is64) != ignore_index;
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) n += whole_at(labels, r, is64) != ignore_index;
     n = block_sum<1024>(n, lds);
     if (threadIdx.x == 0) *global(out) = (float)(n > 0 ? n : 1);
 }
 
 // One workgroup, a fixed order: the same rows give the same loss.  In 64 bits: a row more costs nothing here.
-__global__ __launch_bounds__(1024) void sum_rows_kernel(const float* row_loss, int64_t rows, const float* denominator, float* out)
+__global__ __launch_bounds__(1024) void sum_rows_kernel(const float* row_loss, int64_t rows, const float* denominator, float count, float* out)
 {
     __shared__ double lds[1024];
     double sum = 0.0;
@@ -1060,7 +1069,7 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* row_loss, i
         __syncthreads();
         if ((int)threadIdx.x < n) lds[threadIdx.x] += lds[threadIdx.x + n];
     }
-    if (threadIdx.x == 0) *global(out) = (float)(lds[0] / (denominator ? (double)*global(denominator) : 1.0));
+    if (threadIdx.x == 0) *global(out) = (float)(lds[0] / (double)(denominator ? *global(denominator) : count));
 }
 
 }  // namespace

@@ -210,6 +210,7 @@ int for_rows(int64_t rows, F launch)
     return 0;
 }
 
+constexpr int64_t kCountedRows = 1024;  // counted by every workgroup: 8 KiB of labels; more are counted by a kernel in front (2 us and a launch)
 constexpr int64_t kMaxTopVocab = 1 << 30;
 constexpr int64_t kMaxDistillVocab = 400000;  // a bit each in LDS, beside a list
 
@@ -249,7 +250,10 @@ int distill_args(const ps_distill_call* c, bool backward, DistillArgs& a)
     a.labels = c->labels;
     a.row_loss = c->row_loss;
     a.stats = c->stats;
-    a.denominator = c->mean ? c->denominator : nullptr;
+    // how many rows a mean is over: all of them, or as many as have a label, counted on the GPU
+    a.denominator = c->mean && c->labels ? c->denominator : nullptr;
+    a.count = c->mean ? (float)std::max<int64_t>(c->rows, 1) : 1.0f;
+    a.count_rows = a.denominator && !backward && c->rows > 0 && c->rows <= kCountedRows;
     a.grad = c->grad;
     a.upstream = c->upstream;
     a.upstream_used = c->upstream_used;
@@ -372,7 +376,7 @@ int ps_distill_loss(const ps_distill_call* call, ps_stream_t stream)
     DistillArgs a;
     if (int rc = distill_args(call, false, a)) return rc;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (call->mean) {
+    if (a.denominator && !a.count_rows) {
         hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, st, call->labels, a.labels_64, a.rows, a.ignore_index, call->denominator);
         PS_HIP(hipGetLastError());
     }
@@ -388,7 +392,7 @@ int ps_distill_loss(const ps_distill_call* call, ps_stream_t stream)
     });
     if (rc) return rc;
     if (call->loss) {
-        hipLaunchKernelGGL(sum_rows_kernel, dim3(1), dim3(1024), 0, st, call->row_loss, a.rows, a.denominator, call->loss);
+        hipLaunchKernelGGL(sum_rows_kernel, dim3(1), dim3(1024), 0, st, call->row_loss, a.rows, a.denominator, a.count, call->loss);
         PS_HIP(hipGetLastError());
     }
     return 0;
@@ -398,13 +402,15 @@ int ps_distill_loss_backward(const ps_distill_call* call, ps_stream_t stream)
 {
     DistillArgs a;
     if (int rc = distill_args(call, true, a)) return rc;
-    return for_rows(a.rows, [&](int64_t first, dim3 grid) {
-        a.first_row = first;
-        with_type(call->dtype, [&](auto t) {
-            typedef decltype(t) T;
-            hipLaunchKernelGGL((distill_backward_kernel<T, 256>), grid, dim3(256), 8u * (unsigned)a.k, static_cast<hipStream_t>(stream), a);
-        });
+    if (a.rows == 0) return 0;
+    // (where the gradient is there already, the workgroups are all it costs)
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, 8 * kCus));
+    with_type(call->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((distill_backward_kernel<T, 256>), grid, dim3(256), 8u * (unsigned)a.k, static_cast<hipStream_t>(stream), a);
     });
+    PS_HIP(hipGetLastError());
+    return 0;
 }
 
 }  // extern "C"
