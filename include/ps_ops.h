@@ -78,9 +78,8 @@ typedef struct ps_top_call {
     int32_t* ids;      /* rows x k */
     float* lse;        /* rows */
     int64_t rows, vocab, row_stride;
+    double temperature;
     int32_t k, dtype;
-    float temperature;
-    int32_t reserved;
 } ps_top_call;
 
 int ps_top_logits(const ps_top_call* call, ps_stream_t stream);
@@ -108,9 +107,9 @@ typedef struct ps_distill_call {
     float* upstream_used;        /* 1: the factor that `grad` was made with (NULL: not wanted) */
     int64_t rows, vocab, row_stride, ids_stride, values_stride, upstream_stride;
     int64_t ignore_index;
+    double temperature;
     int32_t k, dtype, values_dtype, ids_bytes, labels_bytes, mean;
-    float temperature, label_weight, upstream_value;
-    int32_t reserved;
+    float label_weight, upstream_value;
 } ps_distill_call;
 
 /* Loss, and the gradient at `upstream` too where `grad` is given: the logits are read once for both. */

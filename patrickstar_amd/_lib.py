@@ -143,10 +143,9 @@ class ps_top_call(ctypes.Structure):
         ("rows", ctypes.c_int64),
         ("vocab", ctypes.c_int64),
         ("row_stride", ctypes.c_int64),
+        ("temperature", ctypes.c_double),
         ("k", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
-        ("temperature", ctypes.c_float),
-        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -171,16 +170,15 @@ class ps_distill_call(ctypes.Structure):
         ("values_stride", ctypes.c_int64),
         ("upstream_stride", ctypes.c_int64),
         ("ignore_index", ctypes.c_int64),
+        ("temperature", ctypes.c_double),
         ("k", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("values_dtype", ctypes.c_int32),
         ("ids_bytes", ctypes.c_int32),
         ("labels_bytes", ctypes.c_int32),
         ("mean", ctypes.c_int32),
-        ("temperature", ctypes.c_float),
         ("label_weight", ctypes.c_float),
         ("upstream_value", ctypes.c_float),
-        ("reserved", ctypes.c_int32),
     ]
 
 

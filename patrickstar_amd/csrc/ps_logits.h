@@ -13,7 +13,7 @@ namespace {
 // (of lambdas that the kernels call in several places: left to itself the compiler keeps their captures in memory)
 #define PS_INLINE __attribute__((always_inline))
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -25,6 +25,13 @@ __device__ __forceinline__ float row_factor(float m, float c)
 {
     const float size = fabsf(m);
     return size * c < 1e37f || size == __builtin_inff() ? c : 1e36f / size;
+}
+
+// log(sum(exp(z / temperature))) from the row's sum of exponentials under m, which are exp2(bias) times too large.  Rows are compared by
+// differences of these, which are far smaller than they are: once a row, in 64 bits.
+__device__ __forceinline__ double log_sum(float m, float bias, double sum, double temperature)
+{
+    return (double)m / temperature + (log(sum) - 0.6931471805599453 * (double)bias);
 }
 
 // ---------------------------------------------------------------------------------------------------- a row and its parts
@@ -238,7 +245,8 @@ struct TopArgs {
     float* lse;
     int64_t first_row, row_stride;  // first_row: of this launch
     int vocab, k;
-    float factor, temperature;  // log2(e) / temperature
+    float factor;  // log2(e) / temperature
+    double temperature;
 };
 
 // Whole numbers in the order of the values: zeros of both signs alike, NaN above everything, never 0.
@@ -602,7 +610,7 @@ __global__ __launch_bounds__(BLOCK, BLOCK == 512 && NV <= 14 ? 6 : 4) void top_l
         }
         const int n = n_found;
         if (thread == 0) {
-            float lse = c == p.factor ? (mc + __builtin_amdgcn_logf(sum)) * kLn2 : m / p.temperature;
+            float lse = (float)log_sum(m, __builtin_fmaf(m, c, -mc), (double)sum, p.temperature);
             if (!ordinary) {  // the row's largest, NaN being larger than everything: a row of -inf alone has no mass
                 uint64_t first = 0;
                 for (int i = 0; i < n; ++i) first = found[i] > first ? found[i] : first;
@@ -662,7 +670,9 @@ struct DistillArgs {
     int64_t ignore_index;
     int vocab, k;
     int values_dtype;
-    float temperature, label_weight, upstream_value, count;
+    float factor, factor_low;  // log2(e) / temperature is their sum
+    float temperature_f, label_weight, upstream_value, count;
+    double temperature, inv_temperature;
     bool ids_64, labels_64;
     bool count_rows;      // few enough for every workgroup to count them itself
 };
@@ -695,60 +705,99 @@ template <typename F>
 __device__ __forceinline__ auto with_softmaxes(const DistillArgs& p, F f)
 {
     const bool both = p.label_weight != 0.0f && p.label_weight != 1.0f;
-    if (!both || p.temperature == 1.0f) return f(Int<kOne>());
-    if (p.temperature == 2.0f) return f(Int<kSquare>());
+    if (!both || p.temperature == 1.0) return f(Int<kOne>());
+    if (p.temperature == 2.0) return f(Int<kSquare>());
     return f(Int<kTwo>());
 }
 
-// The exponentials of a logit: e at the temperature (at 1 if there is no other), e1 at 1.
+// The exponentials of a logit: e at the temperature (at 1 if there is no other), e1 at 1.  Of fp32 logits the factor is taken in two
+// parts: its rounding, 2^-25 of every exponent, is more than their own.
 struct Exponents {
-    float c, mc, c1, mc1;
+    float c, c_low, mc, c1, c1_low, mc1;
 
     __device__ __forceinline__ Exponents(const DistillArgs& p, float m)
     {
-        c = row_factor(m, p.label_weight == 1.0f ? kLog2e : kLog2e / p.temperature);
+        constexpr float kLog2eLow = 1.9259630e-8f;  // log2(e) = kLog2e + this
+        const float own = p.label_weight == 1.0f ? kLog2e : p.factor, own_low = p.label_weight == 1.0f ? kLog2eLow : p.factor_low;
+        c = row_factor(m, own);
+        c_low = c == own ? own_low : 0.0f;
         mc = m * c;
         c1 = row_factor(m, kLog2e);
+        c1_low = c1 == kLog2e ? kLog2eLow : 0.0f;
         mc1 = m * c1;
     }
-    template <int HOW>
+    template <int HOW, bool LOW>
     __device__ __forceinline__ void of(float z, float& e, float& e1) const
     {
-        e = exp2_fast(__builtin_fmaf(z, c, -mc));
+        e = exp2_fast(__builtin_fmaf(z, c, LOW ? __builtin_fmaf(z, c_low, -mc) : -mc));
         if (HOW == kOne) e1 = e;
         if (HOW == kSquare) e1 = e * e;
-        if (HOW == kTwo) e1 = exp2_fast(__builtin_fmaf(z, c1, -mc1));
+        if (HOW == kTwo) e1 = exp2_fast(__builtin_fmaf(z, c1, LOW ? __builtin_fmaf(z, c1_low, -mc1) : -mc1));
+    }
+    // what exp2(-.) brings sums of e, or e1, to sums of exp((z - m) / temperature)
+    template <bool LOW>
+    __device__ __forceinline__ float bias(float m) const
+    {
+        return __builtin_fmaf(m, c, LOW ? __builtin_fmaf(m, c_low, -mc) : -mc);
+    }
+    template <bool LOW>
+    __device__ __forceinline__ float bias1(float m) const
+    {
+        return __builtin_fmaf(m, c1, LOW ? __builtin_fmaf(m, c1_low, -mc1) : -mc1);
     }
 };
 
-// The teacher's list in LDS: ids, probabilities.  Returns through `mass` their sum (every thread).
-template <int BLOCK>
-__device__ __forceinline__ void load_list(const DistillArgs& p, int64_t r, int* ids, float* prob, float* lds_a, float* lds_b, float& mass)
+// The teacher's list in LDS: ids, probabilities and, if wanted, by how much an entry's logit is above the student's, over the
+// temperature.  `mass`: the probabilities' sum.  Their logarithms are value / temperature less `base` and less log(`norm`).  Where the rest
+// counts, 1 - mass does, and of a student near its teacher nothing but the difference of such numbers is left: for fp32 logits they are
+// made in 64 bits.  (16-bit logits are known to 2^-9 or 2^-12 themselves, and the registers that it takes are a workgroup less on a
+// CU: the loss of 4096 x 30522 took 72 us instead of 54.)
+template <typename T>
+using ListSum = std::conditional_t<sizeof(T) == 4, double, float>;
+
+template <int BLOCK, typename T>
+__device__ __forceinline__ void load_list(const DistillArgs& p, int64_t r, const RowShape<T>& shape, int* ids, float* prob, float* above, float* lds_a,
+                                          ListSum<T>* lds_b, ListSum<T>& mass, float& base, ListSum<T>& norm)
 {
+    const bool rest = p.teacher_lse != nullptr;
+    const float given = rest ? *global(p.teacher_lse + r) : 0.0f;
     float top = -__builtin_inff();
+    ListSum<T> sum = 0;
     for (int i = threadIdx.x; i < p.k; i += BLOCK) {
         const int64_t id = whole_at(p.ids, r * p.ids_stride + i, p.ids_64);
-        const float v = value_at(p.values, r * p.values_stride + i, p.values_dtype) / p.temperature;
+        const float value = value_at(p.values, r * p.values_stride + i, p.values_dtype);
         ids[i] = id < 0 ? -1 : id < p.vocab ? (int)id : -2;  // -2: beyond the vocabulary
-        prob[i] = v;
-        if (id >= 0) top = fmaxf(top, v);
+        prob[i] = value / p.temperature_f;
+        if (above) above[i] = ids[i] >= 0 ? (value - to_float<T>(*global(shape.row + id))) / p.temperature_f : 0.0f;
+        if (id >= 0) top = fmaxf(top, prob[i]);
+        if (rest) {
+            ListSum<T> e = 0;
+            if (id >= 0) {
+                if constexpr (sizeof(T) == 4)
+                    e = exp((double)value * p.inv_temperature - (double)given);
+                else
+                    e = expf(prob[i] - given);
+            }
+            prob[i] = (float)e;
+            sum += e;
+        }
     }
-    const bool rest = p.teacher_lse != nullptr;
-    if (rest)
-        top = *global(p.teacher_lse + r);
-    else
+    if (!rest) {
         top = block_max<BLOCK, float>(top, lds_a);
-    float sum = 0.0f;
-    for (int i = threadIdx.x; i < p.k; i += BLOCK) {  // (a thread's own entries)
-        const float e = ids[i] == -1 ? 0.0f : expf(prob[i] - top);
-        prob[i] = e;
-        sum += e;
+        for (int i = threadIdx.x; i < p.k; i += BLOCK) {  // (a thread's own entries)
+            const float e = ids[i] == -1 ? 0.0f : expf(prob[i] - top);
+            prob[i] = e;
+            sum += e;
+        }
     }
     mass = block_sum<BLOCK>(sum, lds_b);
+    base = rest ? given : top;
+    norm = 1;
     if (!rest) {
-        const float scale = mass > 0.0f ? 1.0f / mass : mass == mass ? 0.0f : mass;
+        norm = mass;
+        const float scale = mass > 0 ? 1.0f / (float)mass : mass == mass ? 0.0f : (float)mass;
         for (int i = threadIdx.x; i < p.k; i += BLOCK) prob[i] *= scale;
-        mass = mass > 0.0f ? 1.0f : mass;
+        mass = mass > 0 ? 1 : mass;
     }
     __syncthreads();
 }
@@ -762,7 +811,7 @@ __device__ __forceinline__ void write_gradient(const DistillArgs& p, int64_t r, 
     constexpr int VE = RowShape<T>::VE;
     T* out = static_cast<T*>(p.grad) + r * (int64_t)p.vocab;
     const bool soft_there = p.label_weight != 1.0f, hard_there = p.label_weight != 0.0f;
-    const float soft = soft_there ? factor * (1.0f - p.label_weight) * p.temperature * s.inv_s : 0.0f;
+    const float soft = soft_there ? factor * (1.0f - p.label_weight) * p.temperature_f * s.inv_s : 0.0f;
     const float hard = hard_there ? factor * p.label_weight * s.inv_s1 : 0.0f;
     const float off = soft_there ? soft * s.coef : 0.0f;
     const Exponents exponents(p, s.m);
@@ -771,7 +820,7 @@ __device__ __forceinline__ void write_gradient(const DistillArgs& p, int64_t r, 
         const float share = how() == kOne ? off + hard : off;
         auto gradient = [&](float z) PS_INLINE {
             float e, e1;
-            exponents.of<how()>(z, e, e1);
+            exponents.of<how(), sizeof(T) == 4>(z, e, e1);
             return __builtin_fmaf(e, share, how() == kOne ? 0.0f : e1 * hard);
         };
         data.each(
@@ -785,13 +834,13 @@ __device__ __forceinline__ void write_gradient(const DistillArgs& p, int64_t r, 
             [&](T x, int at) PS_INLINE { *global(out + at) = from_float<T>(gradient(to_float<T>(x))); });
         __syncthreads();
         const float mass_share = p.teacher_lse != nullptr ? soft : off;
-        const float given = factor * (1.0f - p.label_weight) * p.temperature;
+        const float given = factor * (1.0f - p.label_weight) * p.temperature_f;
         if (soft_there) {
             for (int i = threadIdx.x; i < p.k; i += BLOCK) {
                 const int id = ids[i];
                 if (id < 0) continue;
                 float e, e1;
-                exponents.of<how()>(to_float<T>(*global(shape.row + id)), e, e1);
+                exponents.of<how(), sizeof(T) == 4>(to_float<T>(*global(shape.row + id)), e, e1);
                 float g = __builtin_fmaf(e, mass_share, -given * prob[i]);
                 if (hard_there) g += e1 * hard - (id == label ? factor * p.label_weight : 0.0f);
                 *global(out + id) = from_float<T>(g);
@@ -865,7 +914,7 @@ __device__ __forceinline__ RowSums add_up(const RowData<T, NV, BLOCK>& data, con
 #pragma unroll
             for (int k = 0; k < VE; ++k) {
                 float e, e1;
-                exponents.of<HOW>(to_float<T>(v[k]), e, e1);
+                exponents.of<HOW, sizeof(T) == 4>(to_float<T>(v[k]), e, e1);
                 part += e;
                 if (HOW != kOne) at_1 += e1;
             }
@@ -874,7 +923,7 @@ __device__ __forceinline__ RowSums add_up(const RowData<T, NV, BLOCK>& data, con
         },
         [&](T z, int at) PS_INLINE {
             float e, e1;
-            exponents.of<HOW>(to_float<T>(z), e, e1);
+            exponents.of<HOW, sizeof(T) == 4>(to_float<T>(z), e, e1);
             all += e;
             if (HOW != kOne) at_1 += e1;
             if (REST && !members.has(at)) rest += e;
@@ -890,10 +939,12 @@ __global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
     constexpr int VE = RowShape<T>::VE;
     extern __shared__ uint32_t dynamic[];
     __shared__ float lds[6][BLOCK / 64];
+    __shared__ ListSum<T> lds_list[2][BLOCK / 64];
     const int words = member_words(p.vocab);
     uint32_t* member = dynamic;
     int* ids = reinterpret_cast<int*>(dynamic + words);
     float* prob = reinterpret_cast<float*>(dynamic + words + p.k);
+    float* above = prob + p.k;
     const bool rest = p.teacher_lse != nullptr;
     const bool soft = p.label_weight != 1.0f, hard = p.label_weight != 0.0f;
     const float upstream = p.upstream ? *global(p.upstream) : p.upstream_value;
@@ -928,8 +979,9 @@ __global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
         RowData<T, NV, BLOCK> data;
         data.load(shape);
         for (int i = threadIdx.x; i < words; i += BLOCK) member[i] = 0;
-        float mass;
-        load_list<BLOCK>(p, r, ids, prob, lds[0], lds[1], mass);
+        ListSum<T> mass, norm;
+        float base;
+        load_list<BLOCK>(p, r, shape, ids, prob, above, lds[0], lds_list[0], mass, base, norm);
         const Members<T> members(member, shape);
         for (int i = threadIdx.x; i < p.k; i += BLOCK) {
             const int id = ids[i];
@@ -952,24 +1004,30 @@ __global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
                 const uint32_t bits = members.of_vector(first);
                 if (bits & ((1u << (id - first)) - 1)) continue;
                 const vec v = __builtin_bit_cast(vec, shape.vector_at(number));
+                const auto off_list = [&](float z) PS_INLINE {
+                    float x, x1;
+                    exponents.of<kOne, sizeof(T) == 4>(z, x, x1);
+                    return x;
+                };
 #pragma unroll
                 for (int e = 0; e < VE; ++e)
-                    sum_rest += bits >> e & 1 ? 0.0f : exp2_fast(__builtin_fmaf(to_float<T>(v[e]), exponents.c, -exponents.mc));
+                    sum_rest += bits >> e & 1 ? 0.0f : off_list(to_float<T>(v[e]));
             }
         }
-        // the list's part of the divergence: sum p (log p - log q) without q's normaliser, which sum p takes
+        // The list's part of the divergence: sum p (log p - log q), the two logarithms being value / temperature and z / temperature, each
+        // less its log-sum-exp.  The large ones never meet: sums of the differences here, the difference of the sums below.
+        // With the rest, an fp32 student's sum is that off the list and the list's own, the latter in 64 bits like the teacher's: an error of
+        // the former then counts by how far the two rests are apart, not by itself.
         float term = 0.0f;
-        const bool usual = exponents.c == kLog2e / p.temperature;
+        ListSum<T> sum_list = 0;
         if (soft) {
             for (int i = threadIdx.x; i < p.k; i += BLOCK) {
-                const float pr = prob[i];
-                if (ids[i] >= 0 && pr != 0.0f) {
-                    const float z = to_float<T>(*global(shape.row + ids[i]));
-                    const float log_q = usual ? __builtin_fmaf(z, exponents.c, -exponents.mc) * kLn2 : (z - m) / p.temperature;
-                    term = __builtin_fmaf(pr, logf(pr) - log_q, term);
-                }
+                if (ids[i] < 0) continue;
+                if (prob[i] != 0.0f) term = __builtin_fmaf(prob[i], above[i], term);
+                if (rest && sizeof(T) == 4) sum_list += exp(((double)to_float<T>(*global(shape.row + ids[i])) - (double)m) * p.inv_temperature);
             }
         }
+        if (rest && soft && sizeof(T) == 4) sum_list = block_sum<BLOCK>(sum_list, lds_list[1]);
         sum = wave_sum(sum), sum_rest = wave_sum(sum_rest), sum1 = wave_sum(sum1), term = wave_sum(term);
         if ((threadIdx.x & 63) == 0) {
             lds[0][threadIdx.x >> 6] = sum;
@@ -991,26 +1049,46 @@ __global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
         s.m = m;
         s.inv_s = 1.0f / sum;
         s.inv_s1 = 1.0f / sum1;
-        const float p_rest = fmaxf(1.0f - mass, 0.0f), q_rest = sum_rest * s.inv_s;
-        s.coef = rest ? (p_rest == 0.0f ? 1.0f : 1.0f - p_rest / q_rest) : mass;
-        if (threadIdx.x == 0) {
-            float loss = 0.0f;
+        const ListSum<T> p_rest = rest && mass < 1 ? 1 - mass : 0;
+        const double bias = 0.6931471805599453 * (double)exponents.bias<sizeof(T) == 4>(m);
+        ListSum<T> off_list = sum_rest, everything = sum;  // (of 16-bit logits: both with the bias)
+        if constexpr (sizeof(T) == 4) {
+            off_list = (double)sum_rest * (1.0 - bias * (1.0 - 0.5 * bias));  // (a rounding's, far below 1: to the second order)
+            everything = off_list + sum_list;
+        }
+        s.coef = rest ? (p_rest == 0 ? 1.0f : (float)(off_list - p_rest * everything) / (float)off_list) : (float)mass;
+        if (threadIdx.x < 64) {
+            // the row's logarithms, a lane each
+            const int lane = threadIdx.x;
+            const bool biased = !rest || sizeof(T) == 2;
+            const double z_sum = biased ? (double)sum : (double)everything;
+            const double argument = lane == 0 ? z_sum : lane == 1 ? (double)norm : lane == 2 ? (double)p_rest : lane == 3 ? (double)off_list : lane == 4 ? (double)sum1 : 1.0;
+            const double logarithm = log(argument);
+            const double log_z = of_lane(logarithm, 0), log_norm = of_lane(logarithm, 1), log_p = of_lane(logarithm, 2);
+            const double log_off = of_lane(logarithm, 3), log_1 = of_lane(logarithm, 4);
+            if (lane == 0) {
+            double loss = 0.0;
             if (soft) {
-                float kl = __builtin_fmaf(mass, logf(sum), term);
-                if (rest && p_rest > 0.0f) kl = __builtin_fmaf(p_rest, logf(p_rest) - logf(q_rest), kl);
-                loss = (1.0f - p.label_weight) * p.temperature * p.temperature * kl;
+                double kl = (double)term;
+                if (mass != 0) {
+                    const double lse = (double)m * p.inv_temperature + log_z - (biased ? bias : 0.0);
+                    kl += (double)mass * (lse - (double)base - log_norm);
+                }
+                if (p_rest > 0) kl += (double)p_rest * (log_p + log_z - log_off);
+                if (wrong) kl = __builtin_nan("");
+                loss = (1.0 - (double)p.label_weight) * p.temperature * p.temperature * kl;
             }
             if (hard) {
                 const float z = wrong ? m : to_float<T>(*global(shape.row + label));
-                const float log_q = exponents.c1 == kLog2e ? __builtin_fmaf(z, kLog2e, -exponents.mc1) * kLn2 : z - m;
-                loss = __builtin_fmaf(p.label_weight, logf(sum1) - log_q, loss);
+                loss += (double)p.label_weight * ((double)m + log_1 - 0.6931471805599453 * (double)exponents.bias1<sizeof(T) == 4>(m) - (double)z);
             }
-            *global(p.row_loss + r) = loss;
+            *global(p.row_loss + r) = (float)loss;
             if (p.stats) {
                 *global(p.stats + 4 * r) = s.m;
                 *global(p.stats + 4 * r + 1) = s.inv_s;
                 *global(p.stats + 4 * r + 2) = s.coef;
                 *global(p.stats + 4 * r + 3) = s.inv_s1;
+            }
             }
         }
         if (p.grad) write_gradient<T, NV, BLOCK>(p, r, shape, data, s, upstream * inv_count, ids, prob, label);
@@ -1021,7 +1099,8 @@ template <typename T, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void distill_backward_kernel(DistillArgs p)
 {
     extern __shared__ uint32_t dynamic[];
-    __shared__ float lds[2][BLOCK / 64];
+    __shared__ float lds[BLOCK / 64];
+    __shared__ ListSum<T> lds_list[BLOCK / 64];
     // the gradient that the forward pass made is at this very factor
     if (p.upstream_used && *global(p.upstream) == *global(p.upstream_used)) return;
     int* ids = reinterpret_cast<int*>(dynamic);
@@ -1039,8 +1118,9 @@ __global__ __launch_bounds__(BLOCK) void distill_backward_kernel(DistillArgs p)
         s.inv_s = *global(p.stats + 4 * r + 1);
         s.coef = *global(p.stats + 4 * r + 2);
         s.inv_s1 = *global(p.stats + 4 * r + 3);
-        float mass;
-        load_list<BLOCK>(p, r, ids, prob, lds[0], lds[1], mass);
+        ListSum<T> mass, norm;
+        float base;
+        load_list<BLOCK, T>(p, r, shape, ids, prob, nullptr, lds, lds_list, mass, base, norm);
         RowData<T, 0, BLOCK> data;
         data.load(shape);
         write_gradient<T, 0, BLOCK>(p, r, shape, data, s, *global(p.upstream + r * p.upstream_stride) * inv_count, ids, prob, label);

@@ -225,7 +225,8 @@ int check_rows(int64_t rows, int64_t vocab, int64_t most, int dtype, const void*
     return 0;
 }
 
-bool positive(float t) { return t > 0.0f && std::isfinite(t); }
+// (and not beyond fp32, which the kernels use it in)
+bool positive(double t) { return (float)t > 0.0f && std::isfinite((float)t) && std::isfinite((float)(1.4426950408889634 / t)); }
 
 int distill_args(const ps_distill_call* c, bool backward, DistillArgs& a)
 {
@@ -234,7 +235,7 @@ int distill_args(const ps_distill_call* c, bool backward, DistillArgs& a)
     if (!known(c->values_dtype)) return fail(PS_ERR_BAD_ARG, "values_dtype %d is unknown", c->values_dtype);
     if (c->ids_bytes != 4 && c->ids_bytes != 8) return fail(PS_ERR_BAD_ARG, "ids_bytes = %d", c->ids_bytes);
     if (c->labels && c->labels_bytes != 4 && c->labels_bytes != 8) return fail(PS_ERR_BAD_ARG, "labels_bytes = %d", c->labels_bytes);
-    if (!positive(c->temperature)) return fail(PS_ERR_BAD_ARG, "temperature = %g must be positive", (double)c->temperature);
+    if (!positive(c->temperature)) return fail(PS_ERR_BAD_ARG, "temperature = %g must be positive", c->temperature);
     if (!(c->label_weight >= 0.0f && c->label_weight <= 1.0f))
         return fail(PS_ERR_BAD_ARG, "label_weight = %g is not in 0 .. 1", (double)c->label_weight);
     if (c->label_weight > 0.0f && !c->labels) return fail(PS_ERR_BAD_ARG, "label_weight without labels");
@@ -266,7 +267,11 @@ int distill_args(const ps_distill_call* c, bool backward, DistillArgs& a)
     a.vocab = (int)c->vocab;
     a.k = c->k;
     a.values_dtype = c->values_dtype;
+    a.factor = (float)(1.4426950408889634 / c->temperature);
+    a.factor_low = (float)(1.4426950408889634 / c->temperature - (double)a.factor);
     a.temperature = c->temperature;
+    a.inv_temperature = 1.0 / c->temperature;
+    a.temperature_f = (float)c->temperature;
     a.label_weight = c->label_weight;
     a.upstream_value = c->upstream_value;
     a.ids_64 = c->ids_bytes == 8;
@@ -347,7 +352,7 @@ int ps_top_logits(const ps_top_call* call, ps_stream_t stream)
     if (!call) return fail(PS_ERR_BAD_ARG, "call is NULL");
     if (int rc = check_rows(call->rows, call->vocab, kMaxTopVocab, call->dtype, call->logits, call->k)) return rc;
     if (call->k > call->vocab) return fail(PS_ERR_BAD_ARG, "k = %d is more than the vocabulary of %lld", call->k, (long long)call->vocab);
-    if (!positive(call->temperature)) return fail(PS_ERR_BAD_ARG, "temperature = %g must be positive", (double)call->temperature);
+    if (!positive(call->temperature)) return fail(PS_ERR_BAD_ARG, "temperature = %g must be positive", call->temperature);
     if (call->rows == 0) return 0;
     if (!call->values || !call->ids || !call->lse) return fail(PS_ERR_BAD_ARG, "values, ids or lse is NULL");
     TopArgs a;
@@ -358,7 +363,7 @@ int ps_top_logits(const ps_top_call* call, ps_stream_t stream)
     a.row_stride = call->row_stride;
     a.vocab = (int)call->vocab;
     a.k = call->k;
-    a.factor = (float)(1.4426950408889634 / (double)call->temperature);
+    a.factor = (float)(1.4426950408889634 / call->temperature);
     a.temperature = call->temperature;
     return for_rows(call->rows, [&](int64_t first, dim3 grid) {
         a.first_row = first;
@@ -380,7 +385,7 @@ int ps_distill_loss(const ps_distill_call* call, ps_stream_t stream)
         hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, st, call->labels, a.labels_64, a.rows, a.ignore_index, call->denominator);
         PS_HIP(hipGetLastError());
     }
-    const unsigned lds = 4u * (unsigned)member_words(a.vocab) + 8u * (unsigned)a.k;
+    const unsigned lds = 4u * (unsigned)member_words(a.vocab) + 12u * (unsigned)a.k;
     const int rc = for_rows(a.rows, [&](int64_t first, dim3 grid) {
         a.first_row = first;
         with_type(call->dtype, [&](auto t) {

@@ -374,7 +374,7 @@ PyObject* ps_ops_top(PyObject*, PyObject* const* args, Py_ssize_t n)
             c.vocab = logits.size(1);
             c.row_stride = logits.stride(0);
             c.k = (int32_t)k;
-            c.temperature = (float)temperature;
+            c.temperature = temperature;
             check(library.top(&c, stream_of(logits)), "ps_top_logits");
             return {values, ids, lse};
         });
@@ -414,7 +414,7 @@ ps_distill_call distill_call(const Tensor& logits, const Tensor& ids, const Tens
     element_type(values, c.values_dtype);
     whole(ids, c.ids_bytes);
     c.mean = o.reduction == kMean;
-    c.temperature = (float)o.temperature;
+    c.temperature = o.temperature;
     c.label_weight = (float)o.label_weight;
     return c;
 }

@@ -90,16 +90,26 @@ __device__ __forceinline__ void set_element(typename VecOf<T, V>::type& v, int e
     put<T, V>(v, e, from_float<T>(x));
 }
 
-// A value (32 bits) of another lane of the same 16, as CTRL says, and of one lane for the whole wave.  (All lanes take part.)
+// A value of 32 or 64 bits of another lane of the same 16, as CTRL says, and of one lane for the whole wave.  (All lanes take part.)
+template <typename N>
+struct Words {
+    int w[sizeof(N) / 4];
+};
 template <int CTRL, typename N>
 __device__ __forceinline__ N moved(N v)
 {
-    return __builtin_bit_cast(N, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+    Words<N> x = __builtin_bit_cast(Words<N>, v);
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(N) / 4; ++i) x.w[i] = __builtin_amdgcn_update_dpp(0, x.w[i], CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(N, x);
 }
 template <typename N>
 __device__ __forceinline__ N of_lane(N v, int lane)
 {
-    return __builtin_bit_cast(N, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    Words<N> x = __builtin_bit_cast(Words<N>, v);
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(N) / 4; ++i) x.w[i] = __builtin_amdgcn_readlane(x.w[i], lane);
+    return __builtin_bit_cast(N, x);
 }
 
 }  // namespace
