@@ -259,6 +259,8 @@ __device__ __forceinline__ uint32_t order_of(float x)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+constexpr int kRowParts = 8;  // of a thread's part of a row that is not kept
+
 // A thread's sum of exponentials under its own largest logit so far.
 template <typename T>
 struct OnlineSum {
@@ -275,20 +277,27 @@ struct OnlineSum {
         sum = top == -__builtin_inff() ? sum : sum * exp2_fast(__builtin_fmaf(top, c, -mc));
         top = largest;
     }
+    // The thread's whole part of a row; `parts`, one after another at a distance of BLOCK, are the largest of each of kRowParts runs of
+    // `run` vectors.
     template <int BLOCK>
-    __device__ __forceinline__ void add_row(const RowData<T, 0, BLOCK>& data, const RowShape<T>& s, float factor)
+    __device__ __forceinline__ void add_row(const RowData<T, 0, BLOCK>& data, const RowShape<T>& s, float factor, int run, float* parts)
     {
         constexpr int kAhead = 4;  // vectors on their way at a time
         int v = threadIdx.x;
-        for (; v + (kAhead - 1) * BLOCK < s.vectors; v += kAhead * BLOCK) {
-            raw_t x[kAhead];
+        for (int part = 0; part < kRowParts; ++part) {
+            const int end = s.vectors < (part + 1) * run * BLOCK ? s.vectors : (part + 1) * run * BLOCK;
+            float largest = -__builtin_inff();
+            for (; v + (kAhead - 1) * BLOCK < end; v += kAhead * BLOCK) {
+                raw_t x[kAhead];
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) x[j] = s.vector_at(v + j * BLOCK);
-            add<kAhead>(x, factor);
-        }
-        for (; v < s.vectors; v += BLOCK) {
-            const raw_t x[1] = {s.vector_at(v)};
-            add<1>(x, factor);
+                for (int j = 0; j < kAhead; ++j) x[j] = s.vector_at(v + j * BLOCK);
+                largest = fmaxf(largest, add<kAhead>(x, factor));
+            }
+            for (; v < end; v += BLOCK) {
+                const raw_t x[1] = {s.vector_at(v)};
+                largest = fmaxf(largest, add<1>(x, factor));
+            }
+            parts[part * BLOCK] = largest;
         }
         if (data.lone_at >= 0) {
             const float z = to_float<T>(data.lone);
@@ -304,8 +313,9 @@ struct OnlineSum {
         else if (z != z)  // among nothing but -inf so far, which adds nothing
             sum = z;
     }
+    // (returns the largest of them)
     template <int N>
-    __device__ __forceinline__ void add(const raw_t (&x)[N], float factor)
+    __device__ __forceinline__ float add(const raw_t (&x)[N], float factor)
     {
         Largest<T> largest;
 #pragma unroll
@@ -325,6 +335,7 @@ struct OnlineSum {
             for (int e = 0; e < VE; ++e) all += part(to_float<T>(v[e]), c, mc);
             sum += all;
         }
+        return largest.get();
     }
     // the sum under the row's largest logit instead, whose factor is c
     __device__ __forceinline__ float under(float c, float mc) const
@@ -414,10 +425,11 @@ __global__ __launch_bounds__(BLOCK, BLOCK == 512 && NV <= 14 ? 6 : 4) void top_l
     constexpr int VE = RowShape<T>::VE;
     constexpr int kWaves = BLOCK / 64, kPerWave = kBounds / kWaves;  // (BLOCK <= 1024)
     constexpr int kTopCandidates = BLOCK == 256 ? 512 : 2048;
-    constexpr int kSlots = NV == 0 ? BLOCK : BLOCK == 256 ? 256 : 1024;
+    constexpr int kSlots = NV == 0 ? 2048 : BLOCK == 256 ? 256 : 1024;
     __shared__ uint64_t found[kTopCandidates];
     __shared__ raw_t slots[NV > 0 ? kSlots : 1];  // vectors that hold candidates
-    __shared__ int slot_vector[kSlots];           // their numbers (of a row that is not kept: threads that have candidates)
+    __shared__ int slot_vector[kSlots];           // their numbers (of a row that is not kept: the first one's of a run)
+    __shared__ float part_largest[NV > 0 ? 1 : kRowParts * BLOCK];
     __shared__ uint32_t largest[BLOCK];
     __shared__ int place_of[BLOCK];
     __shared__ uint32_t lds_max[kWaves], lds_min[kWaves];
@@ -431,11 +443,13 @@ __global__ __launch_bounds__(BLOCK, BLOCK == 512 && NV <= 14 ? 6 : 4) void top_l
         const RowShape<T> shape(row, p.vocab);
         RowData<T, NV, BLOCK> data;
         data.load(shape);
-        // A row that is not kept is read once for both: a thread's sum goes by its own largest so far.
+        // A row that is not kept is read once for both: a thread's sum goes by its own largest so far.  Of every thread's part it is kept where
+        // its large elements are.
+        const int each = (shape.vectors + BLOCK - 1) / BLOCK, run = (each + kRowParts - 1) / kRowParts;  // vectors of a thread, of a run of its
         OnlineSum<T> online;
         float my_top;
         if constexpr (NV == 0) {
-            online.add_row(data, shape, p.factor);
+            online.add_row(data, shape, p.factor, run, part_largest + thread);
             my_top = online.top;
         } else {
             my_top = data.largest(shape);
@@ -572,26 +586,32 @@ __global__ __launch_bounds__(BLOCK, BLOCK == 512 && NV <= 14 ? 6 : 4) void top_l
             __syncthreads();
             few = few && n_found <= kTopCandidates;
         } else if (few) {
-            // of a row that is not kept, the vectors of threads that reach the bound are read again, spread over all threads
-            const uint64_t reaches = __ballot(mine >= bound);
-            int at = 0;
-            if (lane == 0 && reaches) at = atomicAdd(&n_slots, __popcll(reaches));
-            at = __builtin_amdgcn_readfirstlane(at) + __popcll(reaches & ((1ull << lane) - 1));
+            // of a row that is not kept, the runs that reach the bound are read again, spread over all threads
             if (mine >= bound) {
-                slot_vector[at] = thread;
+                uint32_t reaches = 0;
+#pragma unroll
+                for (int i = 0; i < kRowParts; ++i) reaches |= part_largest[i * BLOCK + thread] >= limit ? 1u << i : 0u;
+                if (reaches) {
+                    int at = atomicAdd(&n_slots, __popc(reaches));
+                    for (int i = 0; i < kRowParts; ++i)
+                        if (reaches >> i & 1) {
+                            if (at < kSlots) slot_vector[at] = i * run * BLOCK + thread;
+                            ++at;
+                        }
+                }
                 if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of<T>(to_float<T>(data.lone), data.lone_at));
             }
             __syncthreads();
-            const int each = (shape.vectors + BLOCK - 1) / BLOCK;  // vectors of a thread
-            const int items = n_slots * each;
+            few = n_slots <= kSlots;
+            const int items = few ? n_slots * run : 0;
             constexpr int kAhead = 4;  // vectors on their way at a time
             for (int first = thread; first < items; first += kAhead * BLOCK) {
                 raw_t x[kAhead];
                 int v[kAhead];
 #pragma unroll
                 for (int j = 0; j < kAhead; ++j) {
-                    const int i = first + j * BLOCK, slot = i / each;
-                    v[j] = i < items ? (i - slot * each) * BLOCK + slot_vector[slot] : shape.vectors;
+                    const int i = first + j * BLOCK, slot = i / run;
+                    v[j] = i < items ? (i - slot * run) * BLOCK + slot_vector[slot] : shape.vectors;
                     asm volatile("" : "=v"(x[j]));
                     if (v[j] < shape.vectors) x[j] = shape.vector_at(v[j]);
                 }
@@ -600,7 +620,7 @@ __global__ __launch_bounds__(BLOCK, BLOCK == 512 && NV <= 14 ? 6 : 4) void top_l
                     if (v[j] < shape.vectors) keep_of(__builtin_bit_cast(vec, x[j]), shape.element_of(v[j]));
             }
             __syncthreads();
-            few = n_found <= kTopCandidates;
+            few = few && n_found <= kTopCandidates;
         }
         if (!few) {
             __syncthreads();  // everyone has seen how many there were
