@@ -2,7 +2,19 @@
 //
 // One workgroup takes a row of logits at a time.  A row that fits is loaded once, all of its loads in flight together, and stays in
 // the workgroup's registers (in its own type, NV 16-byte vectors a thread) while maximum, sums and gradient are made from it;
-// a longer one (NV = 0) is read again for each of them.
+// a longer one (NV = 0) is read again for each of them (by ps_top_logits once).
+//
+// Memory bounds it as long as little is done for a logit: at 16 bits each, a CU has 13 operations for one while it is read.  So a
+// softmax takes a fused multiply-add, the exponential and an addition; the maximum half an operation; whatever is needed once a row or
+// for a list is kept away from the loops over the row.  Rows of an odd vocabulary start at any element: vectors begin at the first
+// 16-byte boundary (16-byte reads from odd elements reach 4.8 TB/s, from boundaries 6.1).  Registers decide how many rows a CU works
+// on at a time, and that hides what a row waits for: values derived from the row are hidden from the compiler, which would keep them
+// (distillation of 8192 x 50257 took 585 us with, 341 without), and loops over rows too (their invariants took 20 to 40 registers).
+// Measured (GPU time):
+//   top 64 of 8192 x 50257 fp16                                  155 us, 0.83 GB, 5.3 TB/s (133 us for reading it)
+//   top 200 of 500 x 200000 fp32                                  87 us, 0.40 GB, 4.6 TB/s
+//   distillation of 8192 x 50257 fp16, a tenth ignored, loss and gradient  330 us, 1.56 GB, 4.7 TB/s (a copy of such rows: 4.8)
+//   the loss alone of 4096 x 30522 bf16, a fifth ignored          50 us, 0.20 GB, 4.0 TB/s
 #ifndef PS_LOGITS_H
 #define PS_LOGITS_H
 
@@ -352,7 +364,7 @@ __device__ __forceinline__ float number_of(uint32_t order)
     return x;  // (NaN: 0x7FFFFFFF)
 }
 
-constexpr int kBounds = 16;      // that are tried at a time
+constexpr int kBounds = 16;  // that are tried at a time
 
 // Low bits of an order that say nothing: the type's own mantissa is shorter than fp32's by so many.
 template <typename T>
@@ -418,6 +430,9 @@ __device__ __forceinline__ void keep_exactly(const T* row, int vocab, int k, uin
 // 3. A candidate's place is the number of larger ones.
 // Where too many reach the bound (long runs of equal logits), or NaN or infinities are in the row, keep_exactly finds the k-th largest
 // (order, place) bit by bit: all are different, so exactly k reach it.
+// Of 155 us for 8192 x 50257, reading and the sum are 132; the search 10, the vectors 15 to 24, the elements 20, the places 17 (each alone,
+// partly hidden).  Tried: candidates read again from memory (50 us more), a vector's elements one after another by one thread (40
+// more), one wave for all places (25 more), workgroups that have the next row on its way (30 more: they fill the registers).
 template <typename T, int NV, int BLOCK>
 __global__ __launch_bounds__(BLOCK, BLOCK == 512 && NV <= 14 ? 6 : 4) void top_logits_kernel(TopArgs p)
 {
@@ -437,237 +452,235 @@ __global__ __launch_bounds__(BLOCK, BLOCK == 512 && NV <= 14 ? 6 : 4) void top_l
     __shared__ int lds_count[2][kBounds];  // (as many as waves, at least)
     __shared__ int n_found, n_slots;
     const int thread = threadIdx.x, lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+    const int64_t r = p.first_row + blockIdx.x;
+    const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
+    const RowShape<T> shape(row, p.vocab);
+    RowData<T, NV, BLOCK> data;
+    data.load(shape);
+    // A row that is not kept is read once for both: a thread's sum goes by its own largest so far.  Of every thread's part it is kept where
+    // its large elements are.
+    const int each = (shape.vectors + BLOCK - 1) / BLOCK, run = (each + kRowParts - 1) / kRowParts;  // vectors of a thread, of a run of its
+    OnlineSum<T> online;
+    float my_top;
+    if constexpr (NV == 0) {
+        online.add_row(data, shape, p.factor, run, part_largest + thread);
+        my_top = online.top;
+    } else {
+        my_top = data.largest(shape);
+    }
+    const uint32_t mine = order_of(my_top);  // (of a thread without elements: -inf's)
+    largest[thread] = mine;
+    if (thread == 0) n_found = n_slots = 0;
     {
-        const int64_t r = p.first_row + blockIdx.x;
-        const T* row = static_cast<const T*>(p.logits) + r * p.row_stride;
-        const RowShape<T> shape(row, p.vocab);
-        RowData<T, NV, BLOCK> data;
-        data.load(shape);
-        // A row that is not kept is read once for both: a thread's sum goes by its own largest so far.  Of every thread's part it is kept where
-        // its large elements are.
-        const int each = (shape.vectors + BLOCK - 1) / BLOCK, run = (each + kRowParts - 1) / kRowParts;  // vectors of a thread, of a run of its
-        OnlineSum<T> online;
-        float my_top;
-        if constexpr (NV == 0) {
-            online.add_row(data, shape, p.factor, run, part_largest + thread);
-            my_top = online.top;
-        } else {
-            my_top = data.largest(shape);
-        }
-        const uint32_t mine = order_of(my_top);  // (of a thread without elements: -inf's)
-        largest[thread] = mine;
-        if (thread == 0) n_found = n_slots = 0;
-        {
-            const uint32_t hi = wave_max(mine), lo = ~wave_max(~mine);
-            if (lane == 0) lds_max[wave] = hi, lds_min[wave] = lo;
-        }
-        __syncthreads();
-        uint32_t most = lds_max[0], least = lds_min[0];
+        const uint32_t hi = wave_max(mine), lo = ~wave_max(~mine);
+        if (lane == 0) lds_max[wave] = hi, lds_min[wave] = lo;
+    }
+    __syncthreads();
+    uint32_t most = lds_max[0], least = lds_min[0];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) {
-            most = lds_max[w] > most ? lds_max[w] : most;
-            least = lds_min[w] < least ? lds_min[w] : least;
-        }
-        const float m = number_of(most), c = row_factor(m, p.factor), mc = m * c;
-        // the sum of exponentials; NaN where a logit is NaN or infinite
-        float sum = 0.0f;
-        if (NV == 0) {
-            sum = online.under(c, mc);
-        } else {
-            data.hide();
-            data.each(
-                shape,
-                [&](const vec& v, int) PS_INLINE {
-                    float part = 0.0f;
+    for (int w = 1; w < kWaves; ++w) {
+        most = lds_max[w] > most ? lds_max[w] : most;
+        least = lds_min[w] < least ? lds_min[w] : least;
+    }
+    const float m = number_of(most), c = row_factor(m, p.factor), mc = m * c;
+    // the sum of exponentials; NaN where a logit is NaN or infinite
+    float sum = 0.0f;
+    if (NV == 0) {
+        sum = online.under(c, mc);
+    } else {
+        data.hide();
+        data.each(
+            shape,
+            [&](const vec& v, int) PS_INLINE {
+                float part = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) part += exp2_fast(__builtin_fmaf(to_float<T>(v[e]), c, -mc));
-                    sum += part;
-                },
-                [&](T x, int) PS_INLINE { sum += exp2_fast(__builtin_fmaf(to_float<T>(x), c, -mc)); });
-        }
-        sum = wave_sum(sum);
-        if (lane == 0) lds_sum[wave] = sum;
-        // the bound: at least k threads reach `bound`, fewer than k `above`
-        uint32_t bound = least, above = most + (most != 0xFFFFFFFFu);
-        int reach = BLOCK;
-        if (p.k <= BLOCK) {
-            const int enough = p.k + p.k / 4 + 8;
-            int turn = 0;
-            uint32_t others[kWaves];
+                for (int e = 0; e < VE; ++e) part += exp2_fast(__builtin_fmaf(to_float<T>(v[e]), c, -mc));
+                sum += part;
+            },
+            [&](T x, int) PS_INLINE { sum += exp2_fast(__builtin_fmaf(to_float<T>(x), c, -mc)); });
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) lds_sum[wave] = sum;
+    // the bound: at least k threads reach `bound`, fewer than k `above`
+    uint32_t bound = least, above = most + (most != 0xFFFFFFFFu);
+    int reach = BLOCK;
+    if (p.k <= BLOCK) {
+        const int enough = p.k + p.k / 4 + 8;
+        int turn = 0;
+        uint32_t others[kWaves];
 #pragma unroll
-            for (int j = 0; j < kWaves; ++j) others[j] = largest[j * 64 + lane];
-            while (reach > enough && above - bound > 1) {
-                const uint32_t step = (above - bound) / (kBounds + 1), left = (above - bound) % (kBounds + 1);
-                auto tried = [&](uint32_t i) PS_INLINE { return bound + step * (i + 1) + (left * (i + 1)) / (kBounds + 1); };
+        for (int j = 0; j < kWaves; ++j) others[j] = largest[j * 64 + lane];
+        while (reach > enough && above - bound > 1) {
+            const uint32_t step = (above - bound) / (kBounds + 1), left = (above - bound) % (kBounds + 1);
+            auto tried = [&](uint32_t i) PS_INLINE { return bound + step * (i + 1) + (left * (i + 1)) / (kBounds + 1); };
 #pragma unroll
-                for (int i = 0; i < kPerWave; ++i) {
-                    const uint32_t limit = tried(wave * kPerWave + i);
-                    int n = 0;
+            for (int i = 0; i < kPerWave; ++i) {
+                const uint32_t limit = tried(wave * kPerWave + i);
+                int n = 0;
 #pragma unroll
-                    for (int j = 0; j < kWaves; ++j) n += __popcll(__ballot(others[j] >= limit));
-                    if (lane == 0) lds_count[turn][wave * kPerWave + i] = n;
-                }
-                __syncthreads();
-                // the bounds rise, so the ones that k threads reach are the first of them
-                const int count = lds_count[turn][lane & (kBounds - 1)];
-                const int reached = __popcll(__ballot(count >= p.k) & ((1u << kBounds) - 1));
-                const uint32_t new_bound = reached > 0 ? tried(reached - 1) : bound;
-                if (reached < kBounds) above = tried(reached);
-                if (reached > 0) reach = __builtin_amdgcn_readlane(count, reached - 1);
-                bound = new_bound;
-                turn ^= 1;
+                for (int j = 0; j < kWaves; ++j) n += __popcll(__ballot(others[j] >= limit));
+                if (lane == 0) lds_count[turn][wave * kPerWave + i] = n;
             }
+            __syncthreads();
+            // the bounds rise, so the ones that k threads reach are the first of them
+            const int count = lds_count[turn][lane & (kBounds - 1)];
+            const int reached = __popcll(__ballot(count >= p.k) & ((1u << kBounds) - 1));
+            const uint32_t new_bound = reached > 0 ? tried(reached - 1) : bound;
+            if (reached < kBounds) above = tried(reached);
+            if (reached > 0) reach = __builtin_amdgcn_readlane(count, reached - 1);
+            bound = new_bound;
+            turn ^= 1;
         }
-        __syncthreads();
-        sum = lds_sum[0];
+    }
+    __syncthreads();
+    sum = lds_sum[0];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) sum += lds_sum[w];
-        const bool ordinary = sum - sum == 0.0f;
-        auto value_of = [](uint64_t entry) PS_INLINE {
-            const uint32_t order = (uint32_t)(entry >> 32) << kLowBits<T>;
-            return number_of(order & 0x80000000u ? order : order | ((1u << kLowBits<T>) - 1));
-        };
-        auto keep = [&](uint64_t entry) PS_INLINE {
-            const int at = atomicAdd(&n_found, 1);
-            if (at < kTopCandidates) found[at] = entry;
-        };
-        // the elements of a vector that reach the limit: one addition for all of them
-        const float limit = number_of(bound);
-        auto keep_of = [&](const vec& x, int first) PS_INLINE {
+    for (int w = 1; w < kWaves; ++w) sum += lds_sum[w];
+    const bool ordinary = sum - sum == 0.0f;
+    auto value_of = [](uint64_t entry) PS_INLINE {
+        const uint32_t order = (uint32_t)(entry >> 32) << kLowBits<T>;
+        return number_of(order & 0x80000000u ? order : order | ((1u << kLowBits<T>) - 1));
+    };
+    auto keep = [&](uint64_t entry) PS_INLINE {
+        const int at = atomicAdd(&n_found, 1);
+        if (at < kTopCandidates) found[at] = entry;
+    };
+    // the elements of a vector that reach the limit: one addition for all of them
+    const float limit = number_of(bound);
+    auto keep_of = [&](const vec& x, int first) PS_INLINE {
+        uint32_t reaches = 0;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) reaches |= to_float<T>(x[e]) >= limit ? 1u << e : 0u;
+        if (!reaches) return;
+        int at = atomicAdd(&n_found, __popc(reaches));
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            if (!(reaches >> e & 1)) continue;
+            if (at < kTopCandidates) found[at] = entry_of<T>(to_float<T>(x[e]), first + e);
+            ++at;
+        }
+    };
+    bool few = ordinary && p.k <= BLOCK && reach <= 2 * p.k + 64;
+    if (few && NV > 0) {
+        // a thread that reaches the bound leaves those of its vectors that do
+        if (mine >= bound) {
             uint32_t reaches = 0;
 #pragma unroll
-            for (int e = 0; e < VE; ++e) reaches |= to_float<T>(x[e]) >= limit ? 1u << e : 0u;
-            if (!reaches) return;
-            int at = atomicAdd(&n_found, __popc(reaches));
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                if (!(reaches >> e & 1)) continue;
-                if (at < kTopCandidates) found[at] = entry_of<T>(to_float<T>(x[e]), first + e);
-                ++at;
+            for (int i = 0; i < NV; ++i) {
+                Largest<T> top;
+                top.add(data.kept[i]);
+                if (i * BLOCK + thread < shape.vectors && top.get() >= limit) reaches |= 1u << i;
             }
-        };
-        bool few = ordinary && p.k <= BLOCK && reach <= 2 * p.k + 64;
-        if (few && NV > 0) {
-            // a thread that reaches the bound leaves those of its vectors that do
-            if (mine >= bound) {
-                uint32_t reaches = 0;
+            if (reaches) {
+                int at = atomicAdd(&n_slots, __popc(reaches));
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    Largest<T> top;
-                    top.add(data.kept[i]);
-                    if (i * BLOCK + thread < shape.vectors && top.get() >= limit) reaches |= 1u << i;
+                    if (!(reaches >> i & 1)) continue;
+                    if (at < kSlots) slots[at] = data.kept[i], slot_vector[at] = i * BLOCK + thread;
+                    ++at;
                 }
-                if (reaches) {
-                    int at = atomicAdd(&n_slots, __popc(reaches));
+            }
+            if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of<T>(to_float<T>(data.lone), data.lone_at));
+        }
+        __syncthreads();
+        const int n = n_slots;
+        few = n <= kSlots;
+        // an element a thread, and one addition a wave
+        const T* elements = reinterpret_cast<const T*>(slots);
+        for (int first = wave * 64; few && first < n * VE; first += BLOCK) {
+            const int i = first + lane;
+            const float x = i < n * VE ? to_float<T>(elements[i]) : 0.0f;
+            const bool reaches = i < n * VE && x >= limit;
+            const uint64_t all = __ballot(reaches);
+            int at = 0;
+            if (lane == 0 && all) at = atomicAdd(&n_found, __popcll(all));
+            at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
+            if (reaches && at < kTopCandidates) found[at] = entry_of<T>(x, shape.element_of(slot_vector[i / VE]) + i % VE);
+        }
+        __syncthreads();
+        few = few && n_found <= kTopCandidates;
+    } else if (few) {
+        // of a row that is not kept, the runs that reach the bound are read again, spread over all threads
+        if (mine >= bound) {
+            uint32_t reaches = 0;
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) {
-                        if (!(reaches >> i & 1)) continue;
-                        if (at < kSlots) slots[at] = data.kept[i], slot_vector[at] = i * BLOCK + thread;
+            for (int i = 0; i < kRowParts; ++i) reaches |= part_largest[i * BLOCK + thread] >= limit ? 1u << i : 0u;
+            if (reaches) {
+                int at = atomicAdd(&n_slots, __popc(reaches));
+                for (int i = 0; i < kRowParts; ++i)
+                    if (reaches >> i & 1) {
+                        if (at < kSlots) slot_vector[at] = i * run * BLOCK + thread;
                         ++at;
                     }
-                }
-                if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of<T>(to_float<T>(data.lone), data.lone_at));
             }
-            __syncthreads();
-            const int n = n_slots;
-            few = n <= kSlots;
-            // an element a thread, and one addition a wave
-            const T* elements = reinterpret_cast<const T*>(slots);
-            for (int first = wave * 64; few && first < n * VE; first += BLOCK) {
-                const int i = first + lane;
-                const float x = i < n * VE ? to_float<T>(elements[i]) : 0.0f;
-                const bool reaches = i < n * VE && x >= limit;
-                const uint64_t all = __ballot(reaches);
-                int at = 0;
-                if (lane == 0 && all) at = atomicAdd(&n_found, __popcll(all));
-                at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
-                if (reaches && at < kTopCandidates) found[at] = entry_of<T>(x, shape.element_of(slot_vector[i / VE]) + i % VE);
-            }
-            __syncthreads();
-            few = few && n_found <= kTopCandidates;
-        } else if (few) {
-            // of a row that is not kept, the runs that reach the bound are read again, spread over all threads
-            if (mine >= bound) {
-                uint32_t reaches = 0;
-#pragma unroll
-                for (int i = 0; i < kRowParts; ++i) reaches |= part_largest[i * BLOCK + thread] >= limit ? 1u << i : 0u;
-                if (reaches) {
-                    int at = atomicAdd(&n_slots, __popc(reaches));
-                    for (int i = 0; i < kRowParts; ++i)
-                        if (reaches >> i & 1) {
-                            if (at < kSlots) slot_vector[at] = i * run * BLOCK + thread;
-                            ++at;
-                        }
-                }
-                if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of<T>(to_float<T>(data.lone), data.lone_at));
-            }
-            __syncthreads();
-            few = n_slots <= kSlots;
-            const int items = few ? n_slots * run : 0;
-            constexpr int kAhead = 4;  // vectors on their way at a time
-            for (int first = thread; first < items; first += kAhead * BLOCK) {
-                raw_t x[kAhead];
-                int v[kAhead];
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    const int i = first + j * BLOCK, slot = i / run;
-                    v[j] = i < items ? (i - slot * run) * BLOCK + slot_vector[slot] : shape.vectors;
-                    asm volatile("" : "=v"(x[j]));
-                    if (v[j] < shape.vectors) x[j] = shape.vector_at(v[j]);
-                }
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    if (v[j] < shape.vectors) keep_of(__builtin_bit_cast(vec, x[j]), shape.element_of(v[j]));
-            }
-            __syncthreads();
-            few = few && n_found <= kTopCandidates;
+            if (data.lone_at >= 0 && to_float<T>(data.lone) >= limit) keep(entry_of<T>(to_float<T>(data.lone), data.lone_at));
         }
-        if (!few) {
-            __syncthreads();  // everyone has seen how many there were
-            if (thread == 0) n_found = 0;
-            keep_exactly<T, BLOCK>(row, p.vocab, p.k, found, &n_found, lds_count[0]);
-            __syncthreads();
-        }
-        const int n = n_found;
-        if (thread == 0) {
-            float lse = (float)log_sum(m, __builtin_fmaf(m, c, -mc), (double)sum, p.temperature);
-            if (!ordinary) {  // the row's largest, NaN being larger than everything: a row of -inf alone has no mass
-                uint64_t first = 0;
-                for (int i = 0; i < n; ++i) first = found[i] > first ? found[i] : first;
-                lse = (uint32_t)(first >> 32) == 0xFFFFFFFFu >> kLowBits<T> ? __builtin_nanf("") : value_of(first);
+        __syncthreads();
+        few = n_slots <= kSlots;
+        const int items = few ? n_slots * run : 0;
+        constexpr int kAhead = 4;  // vectors on their way at a time
+        for (int first = thread; first < items; first += kAhead * BLOCK) {
+            raw_t x[kAhead];
+            int v[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int i = first + j * BLOCK, slot = i / run;
+                v[j] = i < items ? (i - slot * run) * BLOCK + slot_vector[slot] : shape.vectors;
+                asm volatile("" : "=v"(x[j]));
+                if (v[j] < shape.vectors) x[j] = shape.vector_at(v[j]);
             }
-            *global(p.lse + r) = lse;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (v[j] < shape.vectors) keep_of(__builtin_bit_cast(vec, x[j]), shape.element_of(v[j]));
         }
-        auto write = [&](uint64_t entry, int place) PS_INLINE {
-            const uint32_t at = 0xFFFFFFFFu - (uint32_t)entry;
-            const float x = value_of(entry);
-            T value = from_float<T>(x);
-            if (!(x < 0.0f || x > 0.0f)) value = *global(row + at);  // a zero's sign, a NaN's bits
-            *global(p.ids + r * p.k + place) = (int32_t)at;
-            *global(static_cast<T*>(p.values) + r * p.k + place) = value;
-        };
-        if (n <= BLOCK) {
-            int span = 64;
-            while (span < n) span *= 2;
-            const int slices = BLOCK / span, mine_at = thread & (span - 1), slice = thread / span;
-            place_of[thread] = 0;
-            __syncthreads();
-            const uint64_t entry = mine_at < n ? found[mine_at] : 0;
-            int count = 0;
+        __syncthreads();
+        few = few && n_found <= kTopCandidates;
+    }
+    if (!few) {
+        __syncthreads();  // everyone has seen how many there were
+        if (thread == 0) n_found = 0;
+        keep_exactly<T, BLOCK>(row, p.vocab, p.k, found, &n_found, lds_count[0]);
+        __syncthreads();
+    }
+    const int n = n_found;
+    if (thread == 0) {
+        float lse = (float)log_sum(m, __builtin_fmaf(m, c, -mc), (double)sum, p.temperature);
+        if (!ordinary) {  // the row's largest, NaN being larger than everything: a row of -inf alone has no mass
+            uint64_t first = 0;
+            for (int i = 0; i < n; ++i) first = found[i] > first ? found[i] : first;
+            lse = (uint32_t)(first >> 32) == 0xFFFFFFFFu >> kLowBits<T> ? __builtin_nanf("") : value_of(first);
+        }
+        *global(p.lse + r) = lse;
+    }
+    auto write = [&](uint64_t entry, int place) PS_INLINE {
+        const uint32_t at = 0xFFFFFFFFu - (uint32_t)entry;
+        const float x = value_of(entry);
+        T value = from_float<T>(x);
+        if (!(x < 0.0f || x > 0.0f)) value = *global(row + at);  // a zero's sign, a NaN's bits
+        *global(p.ids + r * p.k + place) = (int32_t)at;
+        *global(static_cast<T*>(p.values) + r * p.k + place) = value;
+    };
+    if (n <= BLOCK) {
+        int span = 64;
+        while (span < n) span *= 2;
+        const int slices = BLOCK / span, mine_at = thread & (span - 1), slice = thread / span;
+        place_of[thread] = 0;
+        __syncthreads();
+        const uint64_t entry = mine_at < n ? found[mine_at] : 0;
+        int count = 0;
 #pragma unroll 4
-            for (int j = slice; j < n; j += slices) count += found[j] > entry;
-            if (mine_at < n && count) atomicAdd(&place_of[mine_at], count);
-            __syncthreads();
-            const int place = place_of[mine_at];
-            if (slice == 0 && mine_at < n && place < p.k) write(entry, place);
-        } else {
-            for (int i = thread; i < n; i += BLOCK) {
-                const uint64_t entry = found[i];
-                int place = 0;
+        for (int j = slice; j < n; j += slices) count += found[j] > entry;
+        if (mine_at < n && count) atomicAdd(&place_of[mine_at], count);
+        __syncthreads();
+        const int place = place_of[mine_at];
+        if (slice == 0 && mine_at < n && place < p.k) write(entry, place);
+    } else {
+        for (int i = thread; i < n; i += BLOCK) {
+            const uint64_t entry = found[i];
+            int place = 0;
 #pragma unroll 4
-                for (int j = 0; j < n; ++j) place += found[j] > entry;
-                if (place < p.k) write(entry, place);
-            }
+            for (int j = 0; j < n; ++j) place += found[j] > entry;
+            if (place < p.k) write(entry, place);
         }
     }
 }
@@ -951,6 +964,9 @@ __device__ __forceinline__ RowSums add_up(const RowData<T, NV, BLOCK>& data, con
     return {all, rest, HOW == kOne ? all : at_1};
 }
 
+// Loss, and the gradient in the same pass over the row: maximum, sums, then exponentials again from the registers (keeping them would
+// take twice the registers).  At the speed of a copy of the rows; the list's part (k entries, 64-bit logarithms on a lane each) runs
+// beside other workgroups' reads.  The gradient's vectors start where the logits' do, at any element of an output row.
 // Dynamic LDS: a bit for every token of the vocabulary (is it on the list?), then the list's ids and probabilities.
 template <typename T, int NV, int BLOCK>
 __global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
@@ -978,115 +994,114 @@ __global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
         if (p.first_row + blockIdx.x == 0 && threadIdx.x == 0) *global(p.denominator) = count;
     }
     const float inv_count = 1.0f / count;
-    {
-        const int64_t r = p.first_row + blockIdx.x;
-        const RowShape<T> shape(static_cast<const T*>(p.logits) + r * p.row_stride, p.vocab);
-        int64_t label = -1;
-        bool wrong = false;
-        if (p.labels) {
-            label = whole_at(p.labels, r, p.labels_64);
-            if (label == p.ignore_index) {
-                if (threadIdx.x == 0) {
-                    *global(p.row_loss + r) = 0.0f;
-                    if (p.stats)
-                        for (int i = 0; i < 4; ++i) *global(p.stats + 4 * r + i) = 0.0f;
-                }
-                if (p.grad) write_zeros<T, NV, BLOCK>(p, r, shape);
-                return;
+    const int64_t r = p.first_row + blockIdx.x;
+    const RowShape<T> shape(static_cast<const T*>(p.logits) + r * p.row_stride, p.vocab);
+    int64_t label = -1;
+    bool wrong = false;
+    if (p.labels) {
+        label = whole_at(p.labels, r, p.labels_64);
+        if (label == p.ignore_index) {
+            if (threadIdx.x == 0) {
+                *global(p.row_loss + r) = 0.0f;
+                if (p.stats)
+                    for (int i = 0; i < 4; ++i) *global(p.stats + 4 * r + i) = 0.0f;
             }
-            if (hard) wrong = label < 0 || label >= p.vocab;
+            if (p.grad) write_zeros<T, NV, BLOCK>(p, r, shape);
+            return;
         }
-        RowData<T, NV, BLOCK> data;
-        data.load(shape);
-        for (int i = threadIdx.x; i < words; i += BLOCK) member[i] = 0;
-        ListSum<T> mass, norm;
-        float base;
-        load_list<BLOCK>(p, r, shape, ids, prob, above, lds[0], lds_list[0], mass, base, norm);
-        const Members<T> members(member, shape);
+        if (hard) wrong = label < 0 || label >= p.vocab;
+    }
+    RowData<T, NV, BLOCK> data;
+    data.load(shape);
+    for (int i = threadIdx.x; i < words; i += BLOCK) member[i] = 0;
+    ListSum<T> mass, norm;
+    float base;
+    load_list<BLOCK>(p, r, shape, ids, prob, above, lds[0], lds_list[0], mass, base, norm);
+    const Members<T> members(member, shape);
+    for (int i = threadIdx.x; i < p.k; i += BLOCK) {
+        const int id = ids[i];
+        wrong |= id >= 0 ? members.add(id) : id == -2;
+    }
+    const float m = block_max<BLOCK, float>(data.largest(shape), lds[2]);  // (a barrier: the members are there)
+    const Exponents exponents(p, m);
+    data.hide();
+    const RowSums sums = with_softmaxes(p, [&](auto how) PS_INLINE {
+        if (rest && soft) return add_up<how(), true, T, NV, BLOCK>(data, shape, exponents, members);
+        return add_up<how(), false, T, NV, BLOCK>(data, shape, exponents, members);
+    });
+    float sum = sums.all, sum_rest = sums.rest, sum1 = sums.at_1;
+    if (rest && soft) {
+        // what is off the list in vectors that hold a token of it: the thread of the first such token sees to it
         for (int i = threadIdx.x; i < p.k; i += BLOCK) {
             const int id = ids[i];
-            wrong |= id >= 0 ? members.add(id) : id == -2;
-        }
-        const float m = block_max<BLOCK, float>(data.largest(shape), lds[2]);  // (a barrier: the members are there)
-        const Exponents exponents(p, m);
-        data.hide();
-        const RowSums sums = with_softmaxes(p, [&](auto how) PS_INLINE {
-            if (rest && soft) return add_up<how(), true, T, NV, BLOCK>(data, shape, exponents, members);
-            return add_up<how(), false, T, NV, BLOCK>(data, shape, exponents, members);
-        });
-        float sum = sums.all, sum_rest = sums.rest, sum1 = sums.at_1;
-        if (rest && soft) {
-            // what is off the list in vectors that hold a token of it: the thread of the first such token sees to it
-            for (int i = threadIdx.x; i < p.k; i += BLOCK) {
-                const int id = ids[i];
-                if (id < shape.head || id >= shape.element_of(shape.vectors)) continue;
-                const int number = (id - shape.head) / VE, first = shape.element_of(number);
-                const uint32_t bits = members.of_vector(first);
-                if (bits & ((1u << (id - first)) - 1)) continue;
-                const vec v = __builtin_bit_cast(vec, shape.vector_at(number));
-                const auto off_list = [&](float z) PS_INLINE {
-                    float x, x1;
-                    exponents.of<kOne, sizeof(T) == 4>(z, x, x1);
-                    return x;
-                };
+            if (id < shape.head || id >= shape.element_of(shape.vectors)) continue;
+            const int number = (id - shape.head) / VE, first = shape.element_of(number);
+            const uint32_t bits = members.of_vector(first);
+            if (bits & ((1u << (id - first)) - 1)) continue;
+            const vec v = __builtin_bit_cast(vec, shape.vector_at(number));
+            const auto off_list = [&](float z) PS_INLINE {
+                float x, x1;
+                exponents.of<kOne, sizeof(T) == 4>(z, x, x1);
+                return x;
+            };
 #pragma unroll
-                for (int e = 0; e < VE; ++e)
-                    sum_rest += bits >> e & 1 ? 0.0f : off_list(to_float<T>(v[e]));
-            }
+            for (int e = 0; e < VE; ++e)
+                sum_rest += bits >> e & 1 ? 0.0f : off_list(to_float<T>(v[e]));
         }
-        // The list's part of the divergence: sum p (log p - log q), the two logarithms being value / temperature and z / temperature, each
-        // less its log-sum-exp.  The large ones never meet: sums of the differences here, the difference of the sums below.
-        // With the rest, an fp32 student's sum is that off the list and the list's own, the latter in 64 bits like the teacher's: an error of
-        // the former then counts by how far the two rests are apart, not by itself.
-        float term = 0.0f;
-        ListSum<T> sum_list = 0;
-        if (soft) {
-            for (int i = threadIdx.x; i < p.k; i += BLOCK) {
-                if (ids[i] < 0) continue;
-                if (prob[i] != 0.0f) term = __builtin_fmaf(prob[i], above[i], term);
-                if (rest && sizeof(T) == 4) sum_list += exp(((double)to_float<T>(*global(shape.row + ids[i])) - (double)m) * p.inv_temperature);
-            }
+    }
+    // The list's part of the divergence: sum p (log p - log q), the two logarithms being value / temperature and z / temperature, each
+    // less its log-sum-exp.  The large ones never meet: sums of the differences here, the difference of the sums below.
+    // With the rest, an fp32 student's sum is that off the list and the list's own, the latter in 64 bits like the teacher's: an error of
+    // the former then counts by how far the two rests are apart, not by itself.
+    float term = 0.0f;
+    ListSum<T> sum_list = 0;
+    if (soft) {
+        for (int i = threadIdx.x; i < p.k; i += BLOCK) {
+            if (ids[i] < 0) continue;
+            if (prob[i] != 0.0f) term = __builtin_fmaf(prob[i], above[i], term);
+            if (rest && sizeof(T) == 4) sum_list += exp(((double)to_float<T>(*global(shape.row + ids[i])) - (double)m) * p.inv_temperature);
         }
-        if (rest && soft && sizeof(T) == 4) sum_list = block_sum<BLOCK>(sum_list, lds_list[1]);
-        sum = wave_sum(sum), sum_rest = wave_sum(sum_rest), sum1 = wave_sum(sum1), term = wave_sum(term);
-        if ((threadIdx.x & 63) == 0) {
-            lds[0][threadIdx.x >> 6] = sum;
-            lds[1][threadIdx.x >> 6] = sum_rest;
-            lds[3][threadIdx.x >> 6] = sum1;
-            lds[4][threadIdx.x >> 6] = term;
-        }
-        wrong = __syncthreads_or(wrong);
-        sum = sum_rest = sum1 = term = 0.0f;
+    }
+    if (rest && soft && sizeof(T) == 4) sum_list = block_sum<BLOCK>(sum_list, lds_list[1]);
+    sum = wave_sum(sum), sum_rest = wave_sum(sum_rest), sum1 = wave_sum(sum1), term = wave_sum(term);
+    if ((threadIdx.x & 63) == 0) {
+        lds[0][threadIdx.x >> 6] = sum;
+        lds[1][threadIdx.x >> 6] = sum_rest;
+        lds[3][threadIdx.x >> 6] = sum1;
+        lds[4][threadIdx.x >> 6] = term;
+    }
+    wrong = __syncthreads_or(wrong);
+    sum = sum_rest = sum1 = term = 0.0f;
 #pragma unroll
-        for (int w = 0; w < BLOCK / 64; ++w) {
-            sum += lds[0][w];
-            sum_rest += lds[1][w];
-            sum1 += lds[3][w];
-            term += lds[4][w];
-        }
-        if (wrong) sum = sum1 = __builtin_nanf("");
-        RowStats s;
-        s.m = m;
-        s.inv_s = 1.0f / sum;
-        s.inv_s1 = 1.0f / sum1;
-        const ListSum<T> p_rest = rest && mass < 1 ? 1 - mass : 0;
-        const double bias = 0.6931471805599453 * (double)exponents.bias<sizeof(T) == 4>(m);
-        ListSum<T> off_list = sum_rest, everything = sum;  // (of 16-bit logits: both with the bias)
-        if constexpr (sizeof(T) == 4) {
-            off_list = (double)sum_rest * (1.0 - bias * (1.0 - 0.5 * bias));  // (a rounding's, far below 1: to the second order)
-            everything = off_list + sum_list;
-        }
-        s.coef = rest ? (p_rest == 0 ? 1.0f : (float)(off_list - p_rest * everything) / (float)off_list) : (float)mass;
-        if (threadIdx.x < 64) {
-            // the row's logarithms, a lane each
-            const int lane = threadIdx.x;
-            const bool biased = !rest || sizeof(T) == 2;
-            const double z_sum = biased ? (double)sum : (double)everything;
-            const double argument = lane == 0 ? z_sum : lane == 1 ? (double)norm : lane == 2 ? (double)p_rest : lane == 3 ? (double)off_list : lane == 4 ? (double)sum1 : 1.0;
-            const double logarithm = log(argument);
-            const double log_z = of_lane(logarithm, 0), log_norm = of_lane(logarithm, 1), log_p = of_lane(logarithm, 2);
-            const double log_off = of_lane(logarithm, 3), log_1 = of_lane(logarithm, 4);
-            if (lane == 0) {
+    for (int w = 0; w < BLOCK / 64; ++w) {
+        sum += lds[0][w];
+        sum_rest += lds[1][w];
+        sum1 += lds[3][w];
+        term += lds[4][w];
+    }
+    if (wrong) sum = sum1 = __builtin_nanf("");
+    RowStats s;
+    s.m = m;
+    s.inv_s = 1.0f / sum;
+    s.inv_s1 = 1.0f / sum1;
+    const ListSum<T> p_rest = rest && mass < 1 ? 1 - mass : 0;
+    const double bias = 0.6931471805599453 * (double)exponents.bias<sizeof(T) == 4>(m);
+    ListSum<T> off_list = sum_rest, everything = sum;  // (of 16-bit logits: both with the bias)
+    if constexpr (sizeof(T) == 4) {
+        off_list = (double)sum_rest * (1.0 - bias * (1.0 - 0.5 * bias));  // (a rounding's, far below 1: to the second order)
+        everything = off_list + sum_list;
+    }
+    s.coef = rest ? (p_rest == 0 ? 1.0f : (float)(off_list - p_rest * everything) / (float)off_list) : (float)mass;
+    if (threadIdx.x < 64) {
+        // the row's logarithms, a lane each
+        const int lane = threadIdx.x;
+        const bool biased = !rest || sizeof(T) == 2;
+        const double z_sum = biased ? (double)sum : (double)everything;
+        const double argument = lane == 0 ? z_sum : lane == 1 ? (double)norm : lane == 2 ? (double)p_rest : lane == 3 ? (double)off_list : lane == 4 ? (double)sum1 : 1.0;
+        const double logarithm = log(argument);
+        const double log_z = of_lane(logarithm, 0), log_norm = of_lane(logarithm, 1), log_p = of_lane(logarithm, 2);
+        const double log_off = of_lane(logarithm, 3), log_1 = of_lane(logarithm, 4);
+        if (lane == 0) {
             double loss = 0.0;
             if (soft) {
                 double kl = (double)term;
@@ -1109,12 +1124,12 @@ __global__ __launch_bounds__(BLOCK, 4) void distill_loss_kernel(DistillArgs p)
                 *global(p.stats + 4 * r + 2) = s.coef;
                 *global(p.stats + 4 * r + 3) = s.inv_s1;
             }
-            }
         }
-        if (p.grad) write_gradient<T, NV, BLOCK>(p, r, shape, data, s, upstream * inv_count, ids, prob, label);
     }
+    if (p.grad) write_gradient<T, NV, BLOCK>(p, r, shape, data, s, upstream * inv_count, ids, prob, label);
 }
 
+// The gradient from the row's stats: one read, one write.  Where the forward pass has made it, a launch of workgroups that end (4 us).
 template <typename T, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void distill_backward_kernel(DistillArgs p)
 {
