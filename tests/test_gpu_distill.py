@@ -418,3 +418,20 @@ def test_refusals():
     ]:
         with pytest.raises(error):
             call()
+
+
+def test_more_than_two_to_the_31_elements():
+    rows, vocab = 43001, 50257
+    z = torch.zeros(rows, vocab, dtype=torch.half, device="cuda")
+    z[-4:] = made((4, vocab), torch.half, 1)
+    assert z.numel() > 2**31
+    whole, part = ps.top_logits(z, 16), ps.top_logits(z[-4:], 16)
+    assert all(torch.equal(a[-4:], b) for a, b in zip(whole, part))
+    ids, values = whole.ids, whole.values
+    z.requires_grad_()
+    options = dict(teacher_lse=whole.logsumexp, reduction="sum", grad_scale=8.0)
+    (g,) = torch.autograd.grad(ps.distill_loss(z, ids, values, **options), z, torch.tensor(8.0, device="cuda"))
+    last = z.detach()[-4:].requires_grad_()
+    options["teacher_lse"] = options["teacher_lse"][-4:]
+    (h,) = torch.autograd.grad(ps.distill_loss(last, ids[-4:], values[-4:], **options), last, torch.tensor(8.0, device="cuda"))
+    assert torch.equal(g[-4:], h)

@@ -365,3 +365,18 @@ def test_refusals():
     ]:
         with pytest.raises(error):
             call()
+
+
+def test_more_than_two_to_the_31_elements():
+    tokens, heads, dim = 140001, 120, 128
+    plan = ps.RotaryPlan(dim)
+    q = torch.empty(tokens, heads, dim, dtype=torch.half, device="cuda")
+    q[-3:] = made((3, heads, dim), torch.half, 1)
+    q[:-3] = 1.0
+    at = torch.arange(tokens, device="cuda")
+    w = 1 + made((dim,), torch.half, 5, 0.2)
+    for whole, part in (
+        (ps.rotate_qk(q, None, at, plan)[0], ps.rotate_qk(q[-3:], None, at[-3:], plan)[0]),
+        (ps.norm_rotate_qk(q, None, w, None, at, plan)[0], ps.norm_rotate_qk(q[-3:], None, w, None, at[-3:], plan)[0]),
+    ):
+        assert whole.numel() > 2**31 and torch.equal(whole[-3:], part)
