@@ -15,6 +15,7 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
@@ -349,6 +350,25 @@ PyObject* ps_ops_heads(PyObject*, PyObject* const* args, Py_ssize_t n)
 
 // ------------------------------------------------------------------------------------------------------ logits
 
+namespace {
+
+// [..., n] as [rows, n].
+Tensor flat(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+
+// The dimensions in front of the last one.
+at::IntArrayRef lead_of(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
+
+// [rows] or [rows, n] as they are in front of the last dimension of `like`, with n behind.
+Tensor spread(const Tensor& t, const Tensor& like)
+{
+    if (like.dim() == 2) return t;
+    std::vector<int64_t> sizes = lead_of(like).vec();
+    if (t.dim() == 2) sizes.push_back(t.size(1));
+    return t.view(sizes);
+}
+
+}  // namespace
+
 // (logits, k, temperature) -> (values, ids, log-sum-exp)
 PyObject* ps_ops_top(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
@@ -358,25 +378,26 @@ PyObject* ps_ops_top(PyObject*, PyObject* const* args, Py_ssize_t n)
     double temperature;
     ps_top_call c = {};
     if (n != 3 || c10::impl::dispatch_mode_enabled() || !plain(args[0], device, logits) || !integer(args[1], 1, PS_MAX_TOP, k) ||
-        !number(args[2], temperature) || !element_type(logits, c.dtype) || logits.dim() != 2 || logits.stride(1) != 1 || logits.size(1) < k ||
-        logits.size(1) > 1 << 30 || !((float)temperature > 0.0f && std::isfinite((float)temperature)))
+        !number(args[2], temperature) || !element_type(logits, c.dtype) || logits.dim() < 1 || logits.numel() == 0 || logits.stride(-1) != 1 || logits.size(-1) < k ||
+        logits.size(-1) > 1 << 30 || !((float)temperature > 0.0f && std::isfinite((float)temperature)))
         Py_RETURN_NONE;
     return guarded([&] {
         const variable_list out = without_gil([&]() -> variable_list {
-            const Tensor values = at::empty({logits.size(0), k}, logits.options().requires_grad(false));
-            const Tensor ids = at::empty({logits.size(0), k}, values.options().dtype(at::kInt));
-            const Tensor lse = at::empty({logits.size(0)}, values.options().dtype(at::kFloat));
-            c.logits = logits.data_ptr();
+            const Tensor rows = flat(logits.detach());
+            const Tensor values = at::empty({rows.size(0), k}, rows.options());
+            const Tensor ids = at::empty({rows.size(0), k}, values.options().dtype(at::kInt));
+            const Tensor lse = at::empty({rows.size(0)}, values.options().dtype(at::kFloat));
+            c.logits = rows.data_ptr();
             c.values = values.data_ptr();
             c.ids = static_cast<int32_t*>(ids.data_ptr());
             c.lse = static_cast<float*>(lse.data_ptr());
-            c.rows = logits.size(0);
-            c.vocab = logits.size(1);
-            c.row_stride = logits.stride(0);
+            c.rows = rows.size(0);
+            c.vocab = rows.size(1);
+            c.row_stride = rows.stride(0);
             c.k = (int32_t)k;
             c.temperature = temperature;
-            check(library.top(&c, stream_of(logits)), "ps_top_logits");
-            return {values, ids, lse};
+            check(library.top(&c, stream_of(rows)), "ps_top_logits");
+            return {spread(values, logits), spread(ids, logits), spread(lse, logits)};
         });
         return tuple_of(out);
     });
@@ -521,12 +542,12 @@ PyObject* ps_ops_distill(PyObject*, PyObject* const* args, Py_ssize_t n)
         !integer(args[8], kMean, kNone, reduction))
         Py_RETURN_NONE;
     o.reduction = (int)reduction;
-    if (logits.dim() != 2 || logits.size(0) < 1 || logits.size(1) < 1 || logits.stride(1) != 1 || !element_type(logits, type) || ids.dim() != 2 ||
-        ids.size(0) != logits.size(0) || ids.size(1) < 1 || ids.size(1) > PS_MAX_TOP || ids.stride(1) != 1 || !whole(ids, bytes) ||
-        values.sizes() != ids.sizes() || values.stride(1) != 1 || !element_type(values, type))
+    if (logits.dim() < 1 || logits.numel() == 0 || logits.stride(-1) != 1 || !element_type(logits, type) || ids.dim() != logits.dim() ||
+        lead_of(ids) != lead_of(logits) || ids.size(-1) < 1 || ids.size(-1) > PS_MAX_TOP || ids.stride(-1) != 1 || !whole(ids, bytes) ||
+        values.sizes() != ids.sizes() || values.stride(-1) != 1 || !element_type(values, type))
         Py_RETURN_NONE;
-    if (lse.defined() && (lse.scalar_type() != at::kFloat || lse.dim() != 1 || lse.size(0) != logits.size(0) || !lse.is_contiguous())) Py_RETURN_NONE;
-    if (labels.defined() && (!whole(labels, bytes) || labels.dim() != 1 || labels.size(0) != logits.size(0) || !labels.is_contiguous())) Py_RETURN_NONE;
+    if (lse.defined() && (lse.scalar_type() != at::kFloat || lse.sizes() != lead_of(logits) || !lse.is_contiguous())) Py_RETURN_NONE;
+    if (labels.defined() && (!whole(labels, bytes) || labels.sizes() != lead_of(logits) || !labels.is_contiguous())) Py_RETURN_NONE;
     if (!(o.label_weight >= 0.0 && o.label_weight <= 1.0) || (o.label_weight > 0.0 && !labels.defined()) ||
         !((float)o.temperature > 0.0f && std::isfinite((float)o.temperature)))
         Py_RETURN_NONE;
@@ -537,9 +558,15 @@ PyObject* ps_ops_distill(PyObject*, PyObject* const* args, Py_ssize_t n)
     }
     return guarded([&] {
         const variable_list out = without_gil([&]() -> variable_list {
-            if (!at::GradMode::is_enabled() || !logits.requires_grad()) return {distill(logits, ids, values, lse, labels, o, false, Ahead())[0]};
-            if (ahead.tensor.defined()) ahead.tensor = ahead.tensor.detach().to(at::kFloat);
-            return {DistillFunction::apply(logits, ids.detach(), values.detach(), maybe(lse.defined() ? lse.detach() : lse), maybe(labels), o, ahead)};
+            Tensor loss;
+            const Tensor rows = flat(logits), listed = flat(ids), given = flat(values.detach());
+            if (!at::GradMode::is_enabled() || !logits.requires_grad()) {
+                loss = distill(rows, listed, given, lse, labels, o, false, Ahead())[0];
+            } else {
+                if (ahead.tensor.defined()) ahead.tensor = ahead.tensor.detach().to(at::kFloat);
+                loss = DistillFunction::apply(rows, listed, given, maybe(lse.defined() ? lse.detach() : lse), maybe(labels), o, ahead);
+            }
+            return {o.reduction == kNone ? spread(loss, logits) : loss};
         });
         return THPVariable_Wrap(out[0]);
     });

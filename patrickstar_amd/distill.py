@@ -77,7 +77,8 @@ def distill_loss(logits, ids, teacher_logits, teacher_lse=None, labels=None, *, 
     a label, makes its row's loss and gradient NaN, which the scaler's overflow probe finds.
 
     ``grad_scale``: the factor that backward is going to arrive with (a number, or a tensor with one element on the GPU), if
-    the caller knows it; the logits are then read once for loss and gradient.  Not with ``reduction="none"``.
+    the caller knows it; the logits are then read once for loss and gradient, whose memory is taken in the forward pass.  Another factor
+    is no error: the gradient is then made in the backward pass.  Not with ``reduction="none"``.
     """
     ops = _lib.load().ops
     if ops is not None:

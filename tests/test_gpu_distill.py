@@ -435,3 +435,24 @@ def test_more_than_two_to_the_31_elements():
     options["teacher_lse"] = options["teacher_lse"][-4:]
     (h,) = torch.autograd.grad(ps.distill_loss(last, ids[-4:], values[-4:], **options), last, torch.tensor(8.0, device="cuda"))
     assert torch.equal(g[-4:], h)
+
+
+@pytest.mark.parametrize("lead", [(), (1,), (6,), (2, 3), (1, 2, 3)])
+def test_any_number_of_dimensions_in_front(lead):
+    z = made((*lead, 700), torch.half, 1).requires_grad_()
+    n = math.prod(lead)
+    values, ids, lse = ps.top_logits(z, 9, 2.0)
+    assert values.shape == ids.shape == (*lead, 9) and lse.shape == lead and not values.requires_grad
+    flat = z.detach().view(n, 700).clone().requires_grad_()
+    for a, b in zip((values, ids, lse), ps.top_logits(flat, 9, 2.0)):
+        assert torch.equal(a.reshape(n, -1), b.view(n, -1))
+    labels = torch.arange(n, device="cuda").view(lead)
+    options = dict(label_weight=0.25, temperature=2.0)
+    for reduction in ("mean", "sum", "none"):
+        loss = ps.distill_loss(z, ids, values, lse, labels, reduction=reduction, **options)
+        want = ps.distill_loss(flat, ids.view(n, 9), values.view(n, 9), lse.view(n), labels.view(n), reduction=reduction, **options)
+        assert loss.shape == (lead if reduction == "none" else ()) and torch.equal(loss.detach().reshape(-1), want.detach().reshape(-1))
+        up = made(loss.shape, torch.float, 4)
+        (g,) = torch.autograd.grad(loss, z, up)
+        (h,) = torch.autograd.grad(want, flat, up.reshape(want.shape))
+        assert g.shape == z.shape and torch.equal(g.reshape(n, 700), h)
