@@ -1,4 +1,4 @@
-"""ctypes binding of libps_adam.so (the C ABI declared in include/ps_adam.h).
+"""ctypes binding of libps_adam.so (the C ABI declared in include/ps_adam.h and include/ps_ops.h).
 
 There is no CPU fallback: if the library has not been built, loading raises.
 """
